@@ -1,7 +1,7 @@
 """ctypes bindings to the gfx950 hot-path library (build/libxpu_playground.so).
 
-The C ABI is declared in include/xpu_runtime.h, include/xpu_kernels.h and
-include/xpu_qwen3.h. Every compute call runs the HIP kernels of
+The C ABI is declared in include/xpu_runtime.h, include/xpu_kernels.h,
+include/xpu_qwen3.h and include/xpu_cache.h. Every compute call runs the HIP kernels of
 build/xpu_kernels.hsaco; there is no CPU fallback: if the library or the code
 object is missing, or no gfx950 device is visible, the calls raise.
 """
@@ -50,6 +50,80 @@ class Qwen3Config(ctypes.Structure):
         ("rope_theta", c_double),
         ("tied", c_uint32),
     ]
+
+
+class Cache(ctypes.Structure):
+    """xpu_cache (include/xpu_cache.h): the pages of a KV cache. k and v are
+    device addresses; without strides the pools are [layers][n_pages]
+    [kv_heads][page_size][head_dim]."""
+
+    _fields_ = [
+        ("dtype", c_int),
+        ("layers", c_uint32),
+        ("kv_heads", c_uint32),
+        ("head_dim", c_uint32),
+        ("page_size", c_uint32),
+        ("n_pages", c_uint32),
+        ("layer_stride", c_uint64),
+        ("page_stride", c_uint64),
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("status", c_void_p),
+    ]
+
+    def __init__(self, dtype, layers, kv_heads, head_dim, page_size, n_pages, k=None, v=None, status=None,
+                 layer_stride=None, page_stride=None):
+        page = kv_heads * page_size * head_dim
+        super().__init__(dtype, layers, kv_heads, head_dim, page_size, n_pages,
+                         n_pages * page if layer_stride is None else layer_stride,
+                         page if page_stride is None else page_stride, k, v, status)
+
+
+class Batch(ctypes.Structure):
+    """xpu_batch (include/xpu_cache.h): sequences with new rows; tables,
+    starts and context are device addresses of uint32."""
+
+    _fields_ = [
+        ("n_seqs", c_uint32),
+        ("rows", c_uint32),
+        ("table_pitch", c_uint32),
+        ("tables", c_void_p),
+        ("starts", c_void_p),
+        ("context", c_void_p),
+    ]
+
+
+class Packed(ctypes.Structure):
+    """xpu_packed (include/xpu_cache.h): packed prompts; q_starts and k_starts
+    are device addresses of n_seqs + 1 uint32. Without strides the rows are
+    dense, without k_starts the keys are the queries' rows, and the scale is
+    head_dim ** -0.5."""
+
+    _fields_ = [
+        ("dtype", c_int),
+        ("heads", c_uint32),
+        ("kv_heads", c_uint32),
+        ("head_dim", c_uint32),
+        ("n_seqs", c_uint32),
+        ("q_rows", c_uint32),
+        ("k_rows", c_uint32),
+        ("scale", c_float),
+        ("q_starts", c_void_p),
+        ("k_starts", c_void_p),
+        ("q_stride", c_uint64),
+        ("k_stride", c_uint64),
+        ("v_stride", c_uint64),
+        ("out_stride", c_uint64),
+    ]
+
+    def __init__(self, dtype, heads, kv_heads, head_dim, n_seqs, q_rows, q_starts, k_rows=None, k_starts=None,
+                 scale=None, q_stride=None, k_stride=None, v_stride=None, out_stride=None):
+        def dense(stride, n):
+            return n * head_dim if stride is None else stride
+
+        super().__init__(dtype, heads, kv_heads, head_dim, n_seqs, q_rows, q_rows if k_rows is None else k_rows,
+                         head_dim ** -0.5 if scale is None else scale, q_starts, k_starts, dense(q_stride, heads),
+                         dense(k_stride, kv_heads), dense(v_stride, kv_heads), dense(out_stride, heads))
 
 
 _lib = None
@@ -139,6 +213,45 @@ def _declare(lib):
         "xpu_synth_tokens": (c_int, [c_void_p, c_uint64, c_uint64, c_uint32]),
         "run_gemv": (c_int, [c_int, POINTER(c_char_p)]),
         "run_gemm": (c_int, [c_int, POINTER(c_char_p)]),
+        "xpu_cache_append": (
+            c_int,
+            [c_void_p, POINTER(Cache), POINTER(Batch), c_uint32, c_void_p, c_uint64, c_void_p, c_uint64],
+        ),
+        "xpu_tree_attention": (
+            c_int,
+            [
+                c_void_p,
+                POINTER(Cache),
+                POINTER(Batch),
+                c_uint32,
+                c_uint32,
+                c_float,
+                c_void_p,
+                c_uint64,
+                c_void_p,
+                c_void_p,
+                c_uint64,
+                c_void_p,
+                c_uint64,
+            ],
+        ),
+        "xpu_tree_attention_workspace": (
+            c_int,
+            [c_void_p, POINTER(Cache), POINTER(Batch), c_uint32, POINTER(c_uint64)],
+        ),
+        "xpu_cache_keep": (c_int, [c_void_p, POINTER(Cache), POINTER(Batch), c_void_p, c_void_p, c_void_p]),
+        "xpu_cache_copy": (c_int, [c_void_p, POINTER(Cache), c_void_p, c_void_p, c_uint32]),
+        "xpu_prompt_attention": (c_int, [c_void_p, POINTER(Packed), c_void_p, c_void_p, c_void_p, c_void_p]),
+        "xpu_pages_create": (c_int, [c_uint32, POINTER(c_void_p)]),
+        "xpu_pages_destroy": (None, [c_void_p]),
+        "xpu_pages_free_count": (c_int, [c_void_p, POINTER(c_uint32)]),
+        "xpu_pages_holders": (c_int, [c_void_p, c_uint32, POINTER(c_uint32)]),
+        "xpu_pages_take": (c_int, [c_void_p, c_uint32, c_void_p]),
+        "xpu_pages_share": (c_int, [c_void_p, c_void_p, c_uint32]),
+        "xpu_pages_release": (c_int, [c_void_p, c_void_p, c_uint32]),
+        "xpu_pages_own": (c_int, [c_void_p, c_void_p, c_uint32, c_void_p, c_void_p, POINTER(c_uint32)]),
+        "xpu_pages_compact": (c_int, [c_void_p, c_void_p, c_void_p, POINTER(c_uint32)]),
+        "xpu_pages_renumber": (c_int, [c_void_p, c_void_p, c_uint32, c_void_p, c_uint32]),
         "xpu_peak_mfma": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_uint32, c_uint32]),
         "xpu_peak_read": (c_int, [c_void_p, c_void_p, c_uint64, c_void_p, c_uint32]),
         "run_peak_compute": (c_int, [c_int, POINTER(c_char_p)]),
@@ -345,6 +458,44 @@ class Runtime:
         rows, cols = ctypes.c_uint32(), ctypes.c_uint32()
         check(self.lib.xpu_gemm_tile(self.handle, m, n, ctypes.byref(rows), ctypes.byref(cols)))
         return rows.value, cols.value
+
+    # ---- the paged cache and the attention over it (include/xpu_cache.h);
+    # row operands are device addresses, dense rows without a stride
+    def cache_append(self, cache: Cache, batch: Batch, layer: int, k: int, v: int, k_stride: int | None = None,
+                     v_stride: int | None = None) -> None:
+        dense = cache.kv_heads * cache.head_dim
+        check(self.lib.xpu_cache_append(self.handle, cache, batch, layer, k, dense if k_stride is None else k_stride,
+                                        v, dense if v_stride is None else v_stride))
+
+    def tree_attention_workspace(self, cache: Cache, batch: Batch, heads: int) -> int:
+        """Bytes of workspace that tree_attention needs for these shapes."""
+        v = c_uint64()
+        check(self.lib.xpu_tree_attention_workspace(self.handle, cache, batch, heads, ctypes.byref(v)))
+        return v.value
+
+    def tree_attention(self, cache: Cache, batch: Batch, layer: int, heads: int, q: int, out: int,
+                       workspace: int | None, workspace_bytes: int, visible: int | None = None,
+                       scale: float | None = None, q_stride: int | None = None, out_stride: int | None = None) -> None:
+        dense = heads * cache.head_dim
+        check(self.lib.xpu_tree_attention(self.handle, cache, batch, layer, heads,
+                                          cache.head_dim ** -0.5 if scale is None else scale, q,
+                                          dense if q_stride is None else q_stride, visible, out,
+                                          dense if out_stride is None else out_stride, workspace, workspace_bytes))
+
+    def cache_keep(self, cache: Cache, batch: Batch, kept: int, counts: int, new_context: int | None = None) -> None:
+        check(self.lib.xpu_cache_keep(self.handle, cache, batch, kept, counts, new_context))
+
+    def cache_copy(self, cache: Cache, src, dst) -> None:
+        """src, dst: page ids on the host (arrays or lists of one length)."""
+        import numpy as np
+
+        s, d = (np.ascontiguousarray(ids, dtype=np.uint32) for ids in (src, dst))
+        if s.ndim != 1 or s.shape != d.shape:
+            raise ValueError("src and dst must be one-dimensional and of one length")
+        check(self.lib.xpu_cache_copy(self.handle, cache, s.ctypes.data, d.ctypes.data, len(s)))
+
+    def prompt_attention(self, packed: Packed, q: int, k: int, v: int, out: int) -> None:
+        check(self.lib.xpu_prompt_attention(self.handle, packed, q, k, v, out))
 
     def fill_uniform(self, dtype: int, ptr: int, count: int, seed: int) -> None:
         check(self.lib.xpu_fill_uniform(self.handle, dtype, c_void_p(ptr), count, seed))

@@ -1,0 +1,239 @@
+// What the packed-prompt and the paged-cache attention share: one wavefront's
+// R sub-tiles of 32 query rows against a tile of 32 T keys in LDS.
+//
+//   S^T = K Q^T      A operand: K rows from LDS, B operand: the wave's Q rows,
+//                    held in registers; 32 x 32 tiles, so a lane has the
+//                    scores of ONE query (lane % 32) for 16 T keys
+//   online softmax   per query a reference m, p = 2^((s - m) scale log2 e),
+//                    the FP32 sum of p, and the FP32 output columns; m moves
+//                    (and sum and output are rescaled) only when a score
+//                    passes it by more than 8 in the exponent, so p <= 256
+//                    and rescales are rare after the first tiles
+//   O^T += V^T P^T   B operand: the lane's own p, rounded to the storage type
+//                    where the MFMA reads it (the only rounding between the
+//                    inputs and the result's own), A operand: V^T by the
+//                    transposing LDS read
+//
+// Register r of a 32 x 32 accumulator holds row 8 (r / 4) + 4 (lane / 32) +
+// r % 4, so the keys of a lane's p are 4 hh .. 4 hh + 3 of every 8; the V^T
+// reads take their rows in that order, and no lane exchange is needed.
+//
+// LDS tiles: key rows of 2 D bytes in 16-byte chunks, swizzled so that the
+// K reads (32 rows, one chunk) and the V reads (4 rows, 4 chunks per half
+// wave) each cover every bank once.
+#pragma once
+#include "device_common.hpp"
+
+namespace xpu {
+namespace att {
+
+using dma::f32x16;
+using dma::lds_s16x4;
+
+constexpr float kLazy = 8.0f;  // rescale when the maximum grows by more, in powers of two
+
+// Physical chunk = chunk ^ swizzle(row).
+template <int D> XPU_DEVICE uint32_t k_swz(uint32_t row) {
+  if constexpr (D == 128) return row & 15u;  // 256-byte rows: 16 chunks
+  else return (row >> 1) & 7u;               // 128-byte rows: two rows cover the banks
+}
+template <int D> XPU_DEVICE uint32_t v_swz(uint32_t row) {
+  if constexpr (D == 128) return dma::b_swz(row & 3u);
+  else return (row & 2u) ? 4u : 0u;
+}
+
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) u32x2 lds_u32x2;
+typedef __attribute__((address_space(3))) uint16_t lds_u16;
+
+// Whether a 32-bit word holds an infinity or NaN of the 16-bit type.
+template <int DT> XPU_DEVICE bool nonfinite(uint32_t w) {
+  constexpr uint32_t e = DT == kFp16 ? 0x7c00u : 0x7f80u;
+  return (w & e) == e || (w & (e << 16)) == (e << 16);
+}
+
+// One wavefront's queries. R: sub-tiles of 32 rows.
+template <int DT, int D, int R> struct Rows {
+  static_assert(D == 64 || D == 128, "head sizes");
+  static constexpr int kKs = D / 16, kDt = D / 32;
+  static constexpr uint32_t kRow = 2u * D;  // bytes of a key row
+  u32x4 q[R][kKs];
+  f32x16 o[R][kDt];
+  float m[R], sum[R];
+  uint32_t ka[kKs], va[kDt];  // the lane's LDS offsets in a K and a V tile
+
+  XPU_DEVICE void init() {
+    const uint32_t lane = lane_id(), hh = lane >> 5;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      m[r] = -__builtin_inff();
+      sum[r] = 0.0f;
+#pragma unroll
+      for (int dt = 0; dt < kDt; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[r][dt][i] = 0.0f;
+    }
+    const uint32_t row = lane & 31u;
+#pragma unroll
+    for (uint32_t ks = 0; ks < kKs; ++ks) ka[ks] = row * kRow + 16u * ((2u * ks + hh) ^ k_swz<D>(row));
+    // the transposing read: lane i of a 16-lane group gives row (i % 16) / 4
+    // of the group's 4 rows, dims 16 ((lane / 16) % 2) + 4 (lane % 4)
+    const uint32_t tr_row = (lane & 15u) >> 2, tr_chunk = 2u * ((lane >> 4) & 1u) + ((lane & 3u) >> 1);
+#pragma unroll
+    for (uint32_t dt = 0; dt < kDt; ++dt)
+      va[dt] = (4u * hh + tr_row) * kRow + 16u * ((4u * dt + tr_chunk) ^ v_swz<D>(tr_row)) + 8u * (lane & 1u);
+  }
+
+  // Q row of sub-tile r: dims 16 ks + 8 hh .. + 7 in every ks
+  XPU_DEVICE void load_q(int r, const uint16_t *row) {
+    const uint32_t hh = lane_id() >> 5;
+#pragma unroll
+    for (uint32_t ks = 0; ks < kKs; ++ks) q[r][ks] = *reinterpret_cast<const u32x4 *>(row + (2u * ks + hh) * 8u);
+  }
+
+  // S^T of a tile of 32 T keys at LDS byte address kb.
+  template <int T> XPU_DEVICE void scores(uint32_t kb, f32x16 (&s)[R][T]) const {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[r][t][i] = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < kKs; ++ks)
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        const u32x4 kf = *reinterpret_cast<const lds_u32x4 *>(kb + ka[ks] + 32u * t * kRow);
+#pragma unroll
+        for (int r = 0; r < R; ++r) s[r][t] = dma::mfma<DT>(kf, q[r][ks], s[r][t]);
+      }
+  }
+
+  // Scores of keys that the query does not see: bit k of seen[t] is key
+  // 32 t + k of the tile.
+  template <int T> XPU_DEVICE static void mask(f32x16 (&s)[T], const uint32_t (&seen)[T]) {
+    const uint32_t shift = 4u * (lane_id() >> 5);
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      const uint32_t w = seen[t] >> shift;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (!(w >> (8 * (i / 4) + i % 4) & 1u)) s[t][i] = -__builtin_inff();
+    }
+  }
+
+  // The running maximum, and p of the tile packed as the MFMA takes it:
+  // pk[t][i] holds registers 2 i and 2 i + 1. c = scale log2 e > 0.
+  template <int T> XPU_DEVICE void softmax(int r, const f32x16 (&s)[T], float c, uint32_t (&pk)[T][8]) {
+    const float ninf = -__builtin_inff();
+    float top = ninf;
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
+    top = fmaxf(top, xor32_f(top));  // the query's other half-wave
+    const bool grow = (top - m[r]) * c > kLazy;  // m = -inf: any finite score
+    if (__builtin_amdgcn_ballot_w64(grow)) {
+      const float now = grow ? top : m[r];
+      const float a = m[r] == ninf ? 0.0f : __builtin_amdgcn_exp2f((m[r] - now) * c);
+      sum[r] *= a;
+#pragma unroll
+      for (int dt = 0; dt < kDt; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[r][dt][i] *= a;
+      m[r] = now;
+    }
+    const float shift = m[r] == ninf ? 0.0f : -m[r] * c;  // no score yet: every p is 0
+    float part = 0.0f;
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], c, shift));
+        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i + 1], c, shift));
+        part = part + e0 + e1;
+        pk[t][i / 2] = dma::cvt_pack<DT>(e0, e1);
+      }
+    sum[r] += part;
+  }
+
+  // O^T += V^T P^T for the tile at LDS byte address vb.
+  template <int T> XPU_DEVICE void values(uint32_t vb, const uint32_t (&pk)[R][T][8]) {
+#pragma unroll
+    for (uint32_t ks = 0; ks < 2 * T; ++ks)
+#pragma unroll
+      for (uint32_t dt = 0; dt < kDt; ++dt) {
+        const uint32_t at = vb + va[dt] + 16u * ks * kRow;
+        const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at)));
+        const u32x2 hi =
+            __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at + 8u * kRow)));
+        const u32x4 vf = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const uint32_t(&p)[8] = pk[r][ks / 2];
+          const uint32_t b = 4u * (ks % 2);
+          o[r][dt] = dma::mfma<DT>(vf, u32x4{p[b], p[b + 1], p[b + 2], p[b + 3]}, o[r][dt]);
+        }
+      }
+  }
+
+  // The same for a tile with a non-finite value in a row that some query does
+  // not see: there the product 0 * inf of the MFMA would reach that query, so
+  // each key is added to the queries that see it. One key at a time, p
+  // through 2 KiB of LDS that belong to the wavefront.
+  template <int T>
+  XPU_DEVICE void values_apart(uint32_t vb, int r, const uint32_t (&pk)[T][8], const uint32_t (&seen)[T],
+                               uint32_t scratch) {
+    const uint32_t lane = lane_id(), hh = lane >> 5, query = lane & 31u;
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+#pragma unroll
+      for (uint32_t i = 0; i < 16; ++i)
+        *reinterpret_cast<lds_u16 *>(scratch + ((8u * (i / 4u) + 4u * hh + i % 4u) * 32u + query) * 2u) =
+            static_cast<uint16_t>(pk[t][i / 2] >> (16u * (i % 2u)));
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+      for (uint32_t j = 0; j < 32; ++j) {
+        const bool sees = seen[t] >> j & 1u;
+        const float p = decode<DT>(*reinterpret_cast<const lds_u16 *>(scratch + (j * 32u + query) * 2u));
+        const uint32_t row = vb + (32u * t + j) * kRow + 8u * hh;
+#pragma unroll
+        for (uint32_t dt = 0; dt < kDt; ++dt)
+#pragma unroll
+          for (uint32_t w = 0; w < 4; ++w) {
+            const u32x2 v = *reinterpret_cast<const lds_u32x2 *>(row + 16u * ((4u * dt + w) ^ v_swz<D>(j)));
+            const float f[4] = {lo16<DT>(v.x), hi16<DT>(v.x), lo16<DT>(v.y), hi16<DT>(v.y)};
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) {
+              const float old = o[r][dt][4u * w + e];
+              o[r][dt][4u * w + e] = sees ? __builtin_fmaf(p, f[e], old) : old;
+            }
+          }
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+
+  // The sum over both half-waves of each query.
+  XPU_DEVICE float total(int r) const { return sum[r] + xor32_f(sum[r]); }
+
+  // Row of sub-tile r times `by`, rounded to the storage type.
+  XPU_DEVICE void store(int r, uint16_t *row, float by) const {
+    const uint32_t hh = lane_id() >> 5;
+#pragma unroll
+    for (uint32_t dt = 0; dt < kDt; ++dt)
+#pragma unroll
+      for (uint32_t w = 0; w < 4; ++w)
+        *reinterpret_cast<u32x2 *>(row + 32u * dt + 8u * w + 4u * hh) =
+            u32x2{dma::cvt_pack<DT>(o[r][dt][4 * w] * by, o[r][dt][4 * w + 1] * by),
+                  dma::cvt_pack<DT>(o[r][dt][4 * w + 2] * by, o[r][dt][4 * w + 3] * by)};
+  }
+};
+
+// Bits 0 .. last of a 32-key mask (last < 0: none, last >= 31: all).
+XPU_DEVICE uint32_t mask_to(int32_t last) {
+  return last < 0 ? 0u : last >= 31 ? 0xffffffffu : (2u << last) - 1u;
+}
+
+}  // namespace att
+}  // namespace xpu

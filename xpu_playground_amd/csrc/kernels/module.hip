@@ -15,4 +15,7 @@ __device__ uint32_t xpu_stamp_phase[xpu::kPhaseSlots * xpu::kStampRing * xpu::kP
 #include "prefill_attention_rows.hip"
 #include "gemm.hip"
 #include "prefill_attention.hip"
+#include "packed_attention.hip"
+#include "tree_attention.hip"
+#include "cache.hip"
 #include "peak.hip"

@@ -105,9 +105,10 @@ xpu_runtime::~xpu_runtime() {
 }
 
 const xpu::KernelInfo *xpu_runtime::find_exact(const std::string &name) const {
-  for (const auto &k : kernels)
-    if (k.name == name) return &k;
-  return nullptr;
+  // sorted by name when the module was loaded
+  const auto at = std::lower_bound(kernels.begin(), kernels.end(), name,
+                                   [](const xpu::KernelInfo &k, const std::string &n) { return k.name < n; });
+  return at != kernels.end() && at->name == name ? &*at : nullptr;
 }
 
 int xpu_runtime::scratch(uint64_t bytes, void **out) {

@@ -6,6 +6,7 @@
 #include <hip/hip_runtime_api.h>
 
 #include <cstdint>
+#include <exception>
 #include <map>
 #include <memory>
 #include <string>
@@ -16,6 +17,20 @@ namespace xpu {
 int set_error(int code, const std::string &message);
 void clear_error();
 std::string hip_message(hipError_t e, const char *expr, const char *file, int line);
+
+// body() for a C entry point: no C++ exception leaves it (host memory that
+// runs out is an error code).
+template <typename Body> int guarded(const char *name, Body &&body) {
+  try {
+    return body();
+  } catch (const std::exception &e) {
+    try {
+      return set_error(XPU_ERR_DEVICE, std::string(name) + ": " + e.what());
+    } catch (...) {
+      return XPU_ERR_DEVICE;
+    }
+  }
+}
 
 struct Geometry {
   uint32_t grid = 0, block = 0, shared = 0;
