@@ -30,6 +30,8 @@ namespace att {
 using dma::f32x16;
 using dma::lds_s16x4;
 
+typedef uint32_t u32x8 __attribute__((ext_vector_type(8)));
+
 constexpr float kLazy = 8.0f;  // rescale when the maximum grows by more, in powers of two
 
 // Physical chunk = chunk ^ swizzle(row).
@@ -44,7 +46,7 @@ template <int D> XPU_DEVICE uint32_t v_swz(uint32_t row) {
 
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 typedef __attribute__((address_space(3))) u32x2 lds_u32x2;
-typedef __attribute__((address_space(3))) uint16_t lds_u16;
+typedef __attribute__((address_space(3))) uint32_t lds_u32;
 
 // Whether a 32-bit word holds an infinity or NaN of the 16-bit type.
 template <int DT> XPU_DEVICE bool nonfinite(uint32_t w) {
@@ -90,23 +92,48 @@ template <int DT, int D, int R> struct Rows {
 #pragma unroll
     for (uint32_t ks = 0; ks < kKs; ++ks) q[r][ks] = *reinterpret_cast<const u32x4 *>(row + (2u * ks + hh) * 8u);
   }
+  // The same through LDS, for wavefronts that have their queries in common:
+  // 16 bytes per lane for each ks.
+  static constexpr uint32_t kQBytes = kKs * 1024u;  // of a sub-tile
+  XPU_DEVICE static void stage_q(uint32_t to, uint32_t ks, const uint16_t *row) {
+    *reinterpret_cast<lds_u32x4 *>(to + ks * 1024u + lane_id() * 16u) =
+        *reinterpret_cast<const u32x4 *>(row + (2u * ks + (lane_id() >> 5)) * 8u);
+  }
 
-  // S^T of a tile of 32 T keys at LDS byte address kb.
-  template <int T> XPU_DEVICE void scores(uint32_t kb, f32x16 (&s)[R][T]) const {
+  // S^T of sub-tile r and a tile of 32 T keys at LDS byte address kb; Q from
+  // LDS at qb (QLDS) or from the registers. The reads run one step ahead of
+  // the MFMAs; the barriers keep the compiler from moving all of them to the
+  // front, which would take more registers than there are.
+  template <int T, bool QLDS> XPU_DEVICE void scores(int r, uint32_t kb, uint32_t qb, f32x16 (&s)[T]) const {
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int t = 0; t < T; ++t)
 #pragma unroll
-      for (int t = 0; t < T; ++t)
+      for (int i = 0; i < 16; ++i) s[t][i] = 0.0f;
+    constexpr int kStep = 2;  // ks per step
+    u32x4 kf[2][kStep][T], qf[2][kStep];
+    auto read = [&](int step) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[r][t][i] = 0.0f;
+      for (int j = 0; j < kStep; ++j) {
+        const int ks = step * kStep + j;
 #pragma unroll
-    for (int ks = 0; ks < kKs; ++ks)
-#pragma unroll
-      for (int t = 0; t < T; ++t) {
-        const u32x4 kf = *reinterpret_cast<const lds_u32x4 *>(kb + ka[ks] + 32u * t * kRow);
-#pragma unroll
-        for (int r = 0; r < R; ++r) s[r][t] = dma::mfma<DT>(kf, q[r][ks], s[r][t]);
+        for (int t = 0; t < T; ++t)
+          kf[step & 1][j][t] = *reinterpret_cast<const lds_u32x4 *>(kb + ka[ks] + 32u * t * kRow);
+        if constexpr (QLDS)
+          qf[step & 1][j] = *reinterpret_cast<const lds_u32x4 *>(qb + r * kQBytes + ks * 1024u + lane_id() * 16u);
+        else
+          qf[step & 1][j] = q[r][ks];
       }
+    };
+    read(0);
+#pragma unroll
+    for (int step = 0; step < kKs / kStep; ++step) {
+      if (step + 1 < kKs / kStep) read(step + 1);
+#pragma unroll
+      for (int j = 0; j < kStep; ++j)
+#pragma unroll
+        for (int t = 0; t < T; ++t) s[t] = dma::mfma<DT>(kf[step & 1][j][t], qf[step & 1][j], s[t]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
 
   // Scores of keys that the query does not see: bit k of seen[t] is key
@@ -123,8 +150,8 @@ template <int DT, int D, int R> struct Rows {
   }
 
   // The running maximum, and p of the tile packed as the MFMA takes it:
-  // pk[t][i] holds registers 2 i and 2 i + 1. c = scale log2 e > 0.
-  template <int T> XPU_DEVICE void softmax(int r, const f32x16 (&s)[T], float c, uint32_t (&pk)[T][8]) {
+  // word i of pk[t] holds registers 2 i and 2 i + 1. c = scale log2 e > 0.
+  template <int T> XPU_DEVICE void softmax(int r, const f32x16 (&s)[T], float c, u32x8 (&pk)[T]) {
     const float ninf = -__builtin_inff();
     float top = ninf;
 #pragma unroll
@@ -157,61 +184,74 @@ template <int DT, int D, int R> struct Rows {
     sum[r] += part;
   }
 
-  // O^T += V^T P^T for the tile at LDS byte address vb.
-  template <int T> XPU_DEVICE void values(uint32_t vb, const uint32_t (&pk)[R][T][8]) {
-#pragma unroll
-    for (uint32_t ks = 0; ks < 2 * T; ++ks)
+  // O^T += V^T P^T for the tile at LDS byte address vb, the reads one step (16
+  // keys) ahead of the MFMAs.
+  template <int T> XPU_DEVICE void values(uint32_t vb, const u32x8 (&pk)[R][T]) {
+    u32x4 vf[2][kDt];
+    auto read = [&](uint32_t ks) {
 #pragma unroll
       for (uint32_t dt = 0; dt < kDt; ++dt) {
         const uint32_t at = vb + va[dt] + 16u * ks * kRow;
         const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at)));
         const u32x2 hi =
             __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at + 8u * kRow)));
-        const u32x4 vf = {lo.x, lo.y, hi.x, hi.y};
+        vf[ks & 1u][dt] = u32x4{lo.x, lo.y, hi.x, hi.y};
+      }
+    };
+    read(0);
+#pragma unroll
+    for (uint32_t ks = 0; ks < 2 * T; ++ks) {
+      if (ks + 1u < 2 * T) read(ks + 1u);
+#pragma unroll
+      for (uint32_t dt = 0; dt < kDt; ++dt)
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          const uint32_t(&p)[8] = pk[r][ks / 2];
+          const u32x8 &p = pk[r][ks / 2];
           const uint32_t b = 4u * (ks % 2);
-          o[r][dt] = dma::mfma<DT>(vf, u32x4{p[b], p[b + 1], p[b + 2], p[b + 3]}, o[r][dt]);
+          o[r][dt] = dma::mfma<DT>(vf[ks & 1u][dt], u32x4{p[b], p[b + 1], p[b + 2], p[b + 3]}, o[r][dt]);
         }
-      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
 
-  // The same for a tile with a non-finite value in a row that some query does
-  // not see: there the product 0 * inf of the MFMA would reach that query, so
-  // each key is added to the queries that see it. One key at a time, p
-  // through 2 KiB of LDS that belong to the wavefront.
-  template <int T>
-  XPU_DEVICE void values_apart(uint32_t vb, int r, const uint32_t (&pk)[T][8], const uint32_t (&seen)[T],
-                               uint32_t scratch) {
-    const uint32_t lane = lane_id(), hh = lane >> 5, query = lane & 31u;
-#pragma unroll
-    for (int t = 0; t < T; ++t) {
-#pragma unroll
-      for (uint32_t i = 0; i < 16; ++i)
-        *reinterpret_cast<lds_u16 *>(scratch + ((8u * (i / 4u) + 4u * hh + i % 4u) * 32u + query) * 2u) =
-            static_cast<uint16_t>(pk[t][i / 2] >> (16u * (i % 2u)));
-      __builtin_amdgcn_wave_barrier();
+  // A tile with a non-finite value in a row that some query does not see: the
+  // product 0 * inf of the MFMA would reach that query. So the rows that hold
+  // one are added here to the queries that see them, and then cleared
+  // (clear_apart) before values(). Rare; one key at a time.
+  XPU_DEVICE void add_apart(uint32_t vb, int r, u32x8 pk, uint32_t seen) {
+    const uint32_t hh = lane_id() >> 5;
 #pragma unroll 1
-      for (uint32_t j = 0; j < 32; ++j) {
-        const bool sees = seen[t] >> j & 1u;
-        const float p = decode<DT>(*reinterpret_cast<const lds_u16 *>(scratch + (j * 32u + query) * 2u));
-        const uint32_t row = vb + (32u * t + j) * kRow + 8u * hh;
+    for (uint32_t key = 0; key < 32; ++key) {
+      if (!row_apart(vb + key * kRow)) continue;
+      const uint32_t i = 4u * (key / 8u) + key % 4u;
+      const uint32_t own = pk[i / 2u] >> (16u * (i % 2u)) & 0xffffu, other = xor32_u(own);
+      const bool sees = seen >> key & 1u;
+      const float p = sees ? decode<DT>((key >> 2 & 1u) == hh ? own : other) : 0.0f;
+      const uint32_t row = vb + key * kRow + 8u * hh;
 #pragma unroll
-        for (uint32_t dt = 0; dt < kDt; ++dt)
+      for (uint32_t dt = 0; dt < kDt; ++dt)
 #pragma unroll
-          for (uint32_t w = 0; w < 4; ++w) {
-            const u32x2 v = *reinterpret_cast<const lds_u32x2 *>(row + 16u * ((4u * dt + w) ^ v_swz<D>(j)));
-            const float f[4] = {lo16<DT>(v.x), hi16<DT>(v.x), lo16<DT>(v.y), hi16<DT>(v.y)};
-#pragma unroll
-            for (uint32_t e = 0; e < 4; ++e) {
-              const float old = o[r][dt][4u * w + e];
-              o[r][dt][4u * w + e] = sees ? __builtin_fmaf(p, f[e], old) : old;
-            }
-          }
-      }
-      __builtin_amdgcn_wave_barrier();
+        for (uint32_t w = 0; w < 4; ++w) {
+          const u32x2 v = *reinterpret_cast<const lds_u32x2 *>(row + 16u * ((4u * dt + w) ^ v_swz<D>(key)));
+          const uint32_t x = sees ? v.x : 0u, y = sees ? v.y : 0u;
+          o[r][dt][4u * w] = __builtin_fmaf(p, lo16<DT>(x), o[r][dt][4u * w]);
+          o[r][dt][4u * w + 1u] = __builtin_fmaf(p, hi16<DT>(x), o[r][dt][4u * w + 1u]);
+          o[r][dt][4u * w + 2u] = __builtin_fmaf(p, lo16<DT>(y), o[r][dt][4u * w + 2u]);
+          o[r][dt][4u * w + 3u] = __builtin_fmaf(p, hi16<DT>(y), o[r][dt][4u * w + 3u]);
+        }
     }
+  }
+  // Clears the rows with a non-finite value among `n` rows from LDS address at.
+  XPU_DEVICE static void clear_apart(uint32_t at, uint32_t n) {
+    asm volatile("" ::: "memory");
+#pragma unroll 1
+    for (uint32_t i = 0; i < n; ++i)
+      if (row_apart(at + i * kRow)) *reinterpret_cast<lds_u32 *>(at + i * kRow + lane_id() * 4u % kRow) = 0u;
+    asm volatile("" ::: "memory");
+  }
+  XPU_DEVICE static bool row_apart(uint32_t row) {
+    const uint32_t w = *reinterpret_cast<const lds_u32 *>(row + lane_id() * 4u % kRow);
+    return __builtin_amdgcn_ballot_w64(nonfinite<DT>(w)) != 0;
   }
 
   // The sum over both half-waves of each query.

@@ -49,57 +49,71 @@ template <int D> XPU_DEVICE void append(const AppendArgs &a) {
   }
 }
 
-// One wavefront per (layer, kv head, K or V) of a sequence: all kept rows are
-// loaded before the first is stored (up to 64 rows, 512 / D to an
-// instruction), so the moves may overlap in any order.
+// The moves of `count` rows (at most N loads of 512 / D rows each) of one
+// (layer, kv head, K or V): all are loaded before the first is stored, so they
+// may overlap in any order. Branch-free up to the stores, so that the loads
+// are in flight together: rows that do not move read the pool's first element.
+template <int D, int N>
+XPU_DEVICE void move_rows(const KeepArgs &a, uint16_t *pool, const uint32_t *table, const uint32_t *kept,
+                          uint32_t context, uint32_t nodes, uint32_t count) {
+  constexpr uint32_t kRpi = 512u / D, kCpr = D / 8;
+  const uint32_t lane = lane_id();
+  auto element = [&](uint32_t node) {
+    return element_of(a.pool, table, a.batch.table_pitch, static_cast<uint64_t>(context) + node, D);
+  };
+  uint32_t node[N];
+#pragma unroll
+  for (uint32_t i = 0; i < N; ++i) {
+    const uint32_t j = i * kRpi + lane / kCpr;
+    node[i] = kept[j < count ? j : 0u];
+  }
+  u32x4 held[N];
+  uint64_t to[N];
+  bool odd = false;
+#pragma unroll
+  for (uint32_t i = 0; i < N; ++i) {
+    const uint32_t j = i * kRpi + lane / kCpr;
+    const bool moves = j < count && node[i] != j;
+    const uint64_t from = element(node[i] < nodes ? node[i] : 0u), at = element(j);
+    const bool fine = node[i] < nodes && from != kNowhere && at != kNowhere;
+    to[i] = moves && fine ? at : kNowhere;
+    odd |= moves && !fine;
+    held[i] = *reinterpret_cast<const u32x4 *>(pool + (moves && fine ? from : 0u));
+  }
+  if (__builtin_amdgcn_ballot_w64(odd)) report(a.pool);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+  for (uint32_t i = 0; i < N; ++i)
+    if (to[i] != kNowhere) *reinterpret_cast<u32x4 *>(pool + to[i]) = held[i];
+}
+
+// One wavefront per (layer, kv head, K or V) of a sequence.
 template <int D> XPU_DEVICE void keep(const KeepArgs &a) {
-  constexpr uint32_t kRpi = 512u / D, kCpr = D / 8, kMost = 64u / kRpi;
+  constexpr uint32_t kRpi = 512u / D;
   const uint32_t lane = lane_id();
   const uint32_t per = a.pool.layers * a.pool.kv_heads * 2u;
   const uint64_t index = static_cast<uint64_t>(blockIdx.x) * 4u + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t seq = static_cast<uint32_t>(index / per), part = static_cast<uint32_t>(index % per);
   if (seq >= a.batch.n_seqs) return;
-  const uint32_t lo = a.batch.starts[seq], hi = a.batch.starts[seq + 1], context = a.batch.context[seq];
-  uint32_t count = a.counts[seq];
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(a.batch.starts[seq]);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(a.batch.starts[seq + 1]);
+  const uint32_t context = __builtin_amdgcn_readfirstlane(a.batch.context[seq]);
+  const uint32_t count = __builtin_amdgcn_readfirstlane(a.counts[seq]);
   const bool ok = lo <= hi && hi <= a.batch.rows && count <= hi - lo && count <= 64u;
   if (!ok) {
     report(a.pool);
     return;
   }
   if (part == 0 && lane == 0 && a.new_context) a.new_context[seq] = context + count;
+  if (count == 0) return;  // no row to read the first entry of
   const uint32_t head = part / 2u % a.pool.kv_heads, layer = part / 2u / a.pool.kv_heads;
   uint16_t *pool = (part % 2u ? a.pool.v : a.pool.k) + layer * a.pool.layer_stride +
-                   static_cast<uint64_t>(head) * a.pool.page_size * D + lane % kCpr * 8u;
-  const uint32_t *table = a.batch.tables + static_cast<uint64_t>(seq) * a.batch.table_pitch;
-  auto element = [&](uint32_t node) {
-    return element_of(a.pool, table, a.batch.table_pitch, static_cast<uint64_t>(context) + node, D);
-  };
-  u32x4 held[kMost];
-  uint64_t to[kMost];
-  bool odd = false;
-#pragma unroll
-  for (uint32_t i = 0; i < kMost; ++i) {
-    const uint32_t j = i * kRpi + lane / kCpr;
-    to[i] = kNowhere;
-    if (i * kRpi < count && j < count) {
-      const uint32_t node = a.kept[lo + j];
-      if (node != j) {
-        const uint64_t from = node < hi - lo ? element(node) : kNowhere;
-        to[i] = element(j);
-        if (from == kNowhere || to[i] == kNowhere) {
-          to[i] = kNowhere;
-          odd = true;
-        } else {
-          held[i] = *reinterpret_cast<const u32x4 *>(pool + from);
-        }
-      }
-    }
-  }
-  if (__builtin_amdgcn_ballot_w64(odd)) report(a.pool);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-#pragma unroll
-  for (uint32_t i = 0; i < kMost; ++i)
-    if (to[i] != kNowhere) *reinterpret_cast<u32x4 *>(pool + to[i]) = held[i];
+                   static_cast<uint64_t>(head) * a.pool.page_size * D + lane % (D / 8) * 8u;
+  const uint32_t *table = a.batch.tables + static_cast<uint64_t>(seq) * a.batch.table_pitch, *kept = a.kept + lo;
+  // accepted paths are short: few loads where few rows are kept
+  if (count <= 2u * kRpi) move_rows<D, 2>(a, pool, table, kept, context, hi - lo, count);
+  else if (count <= 16u) move_rows<D, 16 / kRpi>(a, pool, table, kept, context, hi - lo, count);
+  else move_rows<D, 64 / kRpi>(a, pool, table, kept, context, hi - lo, count);
 }
 
 // Block (piece, pair, layer and K or V): 256 x 16 x 4 bytes of a page per step.
@@ -111,12 +125,9 @@ XPU_DEVICE void copy(uint32_t chunks) {
   const u32x4 *from = reinterpret_cast<const u32x4 *>(pool + a.src[pair] * a.pool.page_stride);
   u32x4 *to = reinterpret_cast<u32x4 *>(pool + a.dst[pair] * a.pool.page_stride);
   const uint32_t piece = blockIdx.y * 2048u;
-  u32x4 held[8];
+  u32x4 held[8];  // chunks past the end load the last one
 #pragma unroll
-  for (uint32_t i = 0; i < 8; ++i) {
-    const uint32_t c = piece + i * 256u + threadIdx.x;
-    if (c < chunks) held[i] = from[c];
-  }
+  for (uint32_t i = 0; i < 8; ++i) held[i] = from[min(piece + i * 256u + threadIdx.x, chunks - 1u)];
 #pragma unroll
   for (uint32_t i = 0; i < 8; ++i) {
     const uint32_t c = piece + i * 256u + threadIdx.x;

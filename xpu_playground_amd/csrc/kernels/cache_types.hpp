@@ -37,14 +37,13 @@ struct BatchArgs {
 };
 
 // Element offset of position `pos` in a layer (head 0), or kNowhere where the
-// table (of pitch entries) or the pool has no such page.
+// table (of pitch > 0 entries) or the pool has no such page. Without a branch:
+// a load behind one would be waited for before the next is issued.
 constexpr uint64_t kNowhere = ~0ull;
 XPU_BOTH uint64_t element_of(const PoolArgs &p, const uint32_t *table, uint32_t pitch, uint64_t pos, uint32_t d) {
   const uint64_t page = pos >> p.page_shift;
-  if (page >= pitch) return kNowhere;
-  const uint32_t id = table[page];
-  if (id >= p.n_pages) return kNowhere;
-  return id * p.page_stride + (pos & (p.page_size - 1u)) * d;
+  const uint32_t id = table[page < pitch ? page : pitch - 1u];
+  return page < pitch && id < p.n_pages ? id * p.page_stride + (pos & (p.page_size - 1u)) * d : kNowhere;
 }
 
 // A sequence with rows lo .. hi - 1 behind c positions. Lengths that the batch

@@ -31,7 +31,6 @@ template <int DT, int D, int R> XPU_DEVICE void packed_attention(const PackedArg
   constexpr uint32_t kCpr = D / 8;             // 16-byte chunks per key row
   constexpr uint32_t kDma = kKeys / kRpi / 4;  // DMA instructions per wave, K and V each
   __shared__ __align__(1024) uint8_t lds[2 * kStage];
-  __shared__ __align__(16) uint16_t scratch[4][32 * 32];
   __shared__ uint32_t flags[2][4];  // per stage and wave: its V rows hold a non-finite value
 
   const uint32_t tid = threadIdx.x, lane = tid & 63u;
@@ -120,27 +119,40 @@ template <int DT, int D, int R> XPU_DEVICE void packed_attention(const PackedArg
     }
     __syncthreads();
     if (tile + 1 < n_tiles) issue(tile + 1, stage ^ 1u);
-    if (tile >= wave_tiles) continue;
-    f32x16 s[R][2];
-    rows.template scores<2>(kb, s);
-    const bool masked = static_cast<int32_t>(tile * kKeys + kKeys - 1u) > static_cast<int32_t>(t0) + shift;
-    uint32_t pk[R][2][8], seen[R][2];
+    const bool mine = tile < wave_tiles;
+    u32x8 pk[R][2];
+    uint32_t seen[R][2];
+    if (mine) {
+      const bool masked = static_cast<int32_t>(tile * kKeys + kKeys - 1u) > static_cast<int32_t>(t0) + shift;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if (masked) {  // wave-uniform
-        const int32_t last = static_cast<int32_t>(t0 + 32u * r + (lane & 31u)) + shift - static_cast<int32_t>(tile * kKeys);
-        seen[r][0] = mask_to(last);
-        seen[r][1] = mask_to(last - 32);
-        Rows<DT, D, R>::template mask<2>(s[r], seen[r]);
+      for (int r = 0; r < R; ++r) {
+        f32x16 s[2];
+        rows.template scores<2, false>(r, kb, 0, s);
+        seen[r][0] = seen[r][1] = 0xffffffffu;
+        if (masked) {  // wave-uniform
+          const int32_t last =
+              static_cast<int32_t>(t0 + 32u * r + (lane & 31u)) + shift - static_cast<int32_t>(tile * kKeys);
+          seen[r][0] = mask_to(last);
+          seen[r][1] = mask_to(last - 32);
+          Rows<DT, D, R>::template mask<2>(s, seen[r]);
+        }
+        rows.template softmax<2>(r, s, a.scale_log2e, pk[r]);
       }
-      rows.template softmax<2>(r, s[r], a.scale_log2e, pk[r]);
     }
-    if (masked && __builtin_expect(flags[stage][0] | flags[stage][1] | flags[stage][2] | flags[stage][3], 0)) {
+    if (edge && __builtin_expect(flags[stage][0] | flags[stage][1] | flags[stage][2] | flags[stage][3], 0)) {
+      // the same in every wavefront: all read the rows before any clears its own
+      if (mine) {
 #pragma unroll
-      for (int r = 0; r < R; ++r) rows.template values_apart<2>(vb, r, pk[r], seen[r], lds_addr(scratch[wave]));
-    } else {
-      rows.template values<2>(vb, pk);
+        for (int r = 0; r < R; ++r) {
+          rows.add_apart(vb, r, pk[r][0], seen[r][0]);
+          rows.add_apart(vb + kTile / 2u, r, pk[r][1], seen[r][1]);
+        }
+      }
+      __syncthreads();
+      Rows<DT, D, R>::clear_apart(vb + wave * kTile / 4u, kKeys / 4u);
+      __syncthreads();
     }
+    if (mine) rows.template values<2>(vb, pk);
   }
 #pragma unroll
   for (int r = 0; r < R; ++r) {

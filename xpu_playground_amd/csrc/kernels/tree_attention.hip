@@ -66,8 +66,9 @@ template <int R> XPU_DEVICE uint32_t chunk_limit(const TreeArgs &a, uint32_t gro
   return __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(most < a.least ? a.least : most));
 }
 
-// The work items are numbered sequence by sequence: row tile by row tile, and
-// chunk by chunk within it. find() gives the sequence for which `is(first,
+// The work items are numbered sequence by sequence, chunk by chunk, and row
+// tile by row tile within it, so that the row tiles that read the same keys
+// run side by side (and, with 8 kv heads, on one XCD). find() gives the sequence for which `is(first,
 // count, s)` holds, where first .. first + count - 1 are its items.
 struct Place {
   int32_t seq;  // -1: none
@@ -114,8 +115,8 @@ template <int DT, int D, int R> XPU_DEVICE void tree_attention(const TreeArgs &a
   constexpr uint32_t kMerge = 64u * R * (D / 2u) * 4u;  // bytes of one wave's output columns
   constexpr uint32_t kLds = 8u * kTile > 2u * kMerge ? 8u * kTile : 2u * kMerge;
   __shared__ __align__(1024) uint8_t lds[kLds];  // per wave a K and a V tile; then the partial results
-  __shared__ __align__(16) uint16_t scratch[4][32 * 32];
-  __shared__ float meet[2][R][2][64];
+  // the block's queries, then the (max, sum) pairs that its wavefronts exchange
+  __shared__ __align__(16) uint8_t shared_q[R * Rows<DT, D, R>::kQBytes];
 
   const uint32_t tid = threadIdx.x, lane = tid & 63u, hh = lane >> 5;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -128,7 +129,7 @@ template <int DT, int D, int R> XPU_DEVICE void tree_attention(const TreeArgs &a
   if (place.seq < 0) return;
   const uint32_t seq = static_cast<uint32_t>(place.seq);
   const Sequence s = uniform_sequence<R>(a.batch, a.pool.page_size, group, seq);
-  const uint32_t row_tile = (item - place.first) / place.chunks, chunk = (item - place.first) % place.chunks;
+  const uint32_t row_tile = (item - place.first) % s.row_tiles, chunk = (item - place.first) / s.row_tiles;
   const uint32_t rows_in = min(s.n * group - row_tile * 32u * R, 32u * R);
   // the chunk's tiles, and the wave's share of them
   const uint32_t c0 = static_cast<uint32_t>(static_cast<uint64_t>(s.tiles) * chunk / place.chunks);
@@ -145,6 +146,7 @@ template <int DT, int D, int R> XPU_DEVICE void tree_attention(const TreeArgs &a
   uint32_t w_from = t_lo * kTreeKeys >> a.pool.page_shift;
   uint32_t ids = window(w_from), ids_next = window(w_from + 64u);
 
+  const uint32_t qb = __builtin_amdgcn_readfirstlane(lds_addr(shared_q));
   Rows<DT, D, R> rows;
   rows.init();
   uint32_t node[R];
@@ -153,7 +155,10 @@ template <int DT, int D, int R> XPU_DEVICE void tree_attention(const TreeArgs &a
   for (int r = 0; r < R; ++r) {
     const uint32_t row = min(row_tile * 32u * R + 32u * r + (lane & 31u), s.n * group - 1u);
     node[r] = row / group;
-    rows.load_q(r, a.q + (s.first + node[r]) * a.q_stride + (kvh * group + row % group) * D);
+    const uint16_t *q_row = a.q + (s.first + node[r]) * a.q_stride + (kvh * group + row % group) * D;
+#pragma unroll
+    for (uint32_t j = 0; j < D / 64; ++j)
+      Rows<DT, D, R>::stage_q(qb + r * Rows<DT, D, R>::kQBytes, wave * (D / 64u) + j, q_row);
     if (a.visible) {
       sees[r] = a.visible[s.first + node[r]];
       if (s.n < 64u) sees[r] &= (1ull << s.n) - 1ull;
@@ -211,32 +216,33 @@ template <int DT, int D, int R> XPU_DEVICE void tree_attention(const TreeArgs &a
     issue(a.pool.k, kb, k_off, from, live);
     issue(a.pool.v, vb, v_off, from, live);
   }
+  __syncthreads();  // the queries are there
   for (uint32_t tile = t_lo; tile < t_hi; ++tile) {
     const bool more = tile + 1u < t_hi;
     wait_vmcnt<kDma>();  // K is there; V may be on its way
-    f32x16 sc[R][1];
-    rows.template scores<1>(kb, sc);
-    if (more) {
-      locate(tile + 1u);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K is read
-      issue(a.pool.k, kb, k_off, from, live);
-    }
     const int32_t base = static_cast<int32_t>(s.context - tile * kTreeKeys);  // node 0 in the tile
     const bool edge = (tile + 1u) * kTreeKeys > s.context;  // the tile holds nodes (or ends the sequence)
-    uint32_t pk[R][1][8], seen[R][1];
+    u32x8 pk[R][1];
+    uint32_t seen[R][1] = {};
 #pragma unroll
     for (int r = 0; r < R; ++r) {
+      f32x16 sc[1];
+      rows.template scores<1, true>(r, kb, qb, sc);
+      if (r == R - 1 && more) {
+        locate(tile + 1u);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K is read
+        issue(a.pool.k, kb, k_off, from, live);
+      }
       if (edge) {  // wave-uniform
         if (!a.visible) seen[r][0] = mask_to(base + static_cast<int32_t>(node[r]));
         else if (base >= 0) seen[r][0] = static_cast<uint32_t>(sees[r] << base) | ((1u << base) - 1u);
         else seen[r][0] = base > -64 ? static_cast<uint32_t>(sees[r] >> -base) : 0u;
-        Rows<DT, D, R>::template mask<1>(sc[r], seen[r]);
+        Rows<DT, D, R>::template mask<1>(sc, seen[r]);
       }
-      rows.template softmax<1>(r, sc[r], a.scale_log2e, pk[r]);
+      rows.template softmax<1>(r, sc, a.scale_log2e, pk[r]);
     }
     if (more) wait_vmcnt<kDma>();
     else wait_vmcnt<0>();
-    bool apart = false;
     if (edge) {
       bool odd = false;
 #pragma unroll
@@ -244,14 +250,13 @@ template <int DT, int D, int R> XPU_DEVICE void tree_attention(const TreeArgs &a
         const u32x4 w = *reinterpret_cast<const lds_u32x4 *>(vb + j * 1024u + lane * 16u);
         odd |= nonfinite<DT>(w.x) || nonfinite<DT>(w.y) || nonfinite<DT>(w.z) || nonfinite<DT>(w.w);
       }
-      apart = __builtin_amdgcn_ballot_w64(odd) != 0;
-    }
-    if (__builtin_expect(apart, 0)) {
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd) != 0, 0)) {
 #pragma unroll
-      for (int r = 0; r < R; ++r) rows.template values_apart<1>(vb, r, pk[r], seen[r], lds_addr(scratch[wave]));
-    } else {
-      rows.template values<1>(vb, pk);
+        for (int r = 0; r < R; ++r) rows.add_apart(vb, r, pk[r][0], seen[r][0]);
+        Rows<DT, D, R>::clear_apart(vb, kTreeKeys);
+      }
     }
+    rows.template values<1>(vb, pk);
     if (more) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V is read
       issue(a.pool.v, vb, v_off, from, live);
@@ -264,7 +269,7 @@ template <int DT, int D, int R> XPU_DEVICE void tree_attention(const TreeArgs &a
 #pragma unroll
   for (int r = 0; r < R; ++r) sum[r] = bad ? __builtin_nanf("") : rows.total(r);
   if (bad && lane == 0 && a.pool.status) *a.pool.status = 1u;
-  float *po = reinterpret_cast<float *>(lds);
+  float *po = reinterpret_cast<float *>(lds), *meet = reinterpret_cast<float *>(shared_q);
 #pragma unroll
   for (uint32_t half = 2; half; half >>= 1) {
     __syncthreads();
@@ -272,8 +277,8 @@ template <int DT, int D, int R> XPU_DEVICE void tree_attention(const TreeArgs &a
       const uint32_t w = wave - half;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        meet[w][r][0][lane] = rows.m[r];
-        meet[w][r][1][lane] = sum[r];
+        meet[((w * R + r) * 2u) * 64u + lane] = rows.m[r];
+        meet[((w * R + r) * 2u + 1u) * 64u + lane] = sum[r];
 #pragma unroll
         for (uint32_t dt = 0; dt < D / 32; ++dt)
 #pragma unroll
@@ -285,19 +290,21 @@ template <int DT, int D, int R> XPU_DEVICE void tree_attention(const TreeArgs &a
     if (wave < half) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const float m2 = meet[wave][r][0][lane], s2 = meet[wave][r][1][lane];
+        const float m2 = meet[((wave * R + r) * 2u) * 64u + lane], s2 = meet[((wave * R + r) * 2u + 1u) * 64u + lane];
         const float now = fmaxf(rows.m[r], m2), ninf = -__builtin_inff();
         const float x = rows.m[r] == ninf ? 0.0f : __builtin_amdgcn_exp2f((rows.m[r] - now) * a.scale_log2e);
         const float y = m2 == ninf ? 0.0f : __builtin_amdgcn_exp2f((m2 - now) * a.scale_log2e);
         // a side without a finite score has only zeros or NaN, which stay
         sum[r] = (rows.m[r] == ninf ? sum[r] : sum[r] * x) + (m2 == ninf ? s2 : s2 * y);
 #pragma unroll
-        for (uint32_t dt = 0; dt < D / 32; ++dt)
+        for (uint32_t dt = 0; dt < D / 32; ++dt) {
+          __builtin_amdgcn_sched_barrier(0);  // 16 reads at a time: all of them would need the registers of `o` again
 #pragma unroll
           for (uint32_t i = 0; i < 16; ++i) {
             const float o2 = po[((wave * R + r) * (D / 2u) + dt * 16u + i) * 64u + lane];
             rows.o[r][dt][i] = __builtin_fmaf(rows.o[r][dt][i], x, o2 * y);
           }
+        }
         rows.m[r] = now;
       }
     }
@@ -343,8 +350,8 @@ template <int DT, int D, int R> XPU_DEVICE void tree_join(const TreeArgs &a) {
   const Sequence s = uniform_sequence<R>(a.batch, a.pool.page_size, group, static_cast<uint32_t>(place.seq));
   const uint32_t kvh = head / group, row = (row_at - s.first) * group + head % group;
   const uint32_t in = row % (32u * R);
-  const uint64_t step = static_cast<uint64_t>(a.pool.kv_heads) * kPartial<D, R>;
-  const float *part = a.partial + (static_cast<uint64_t>(place.first + row / (32u * R) * place.chunks) * a.pool.kv_heads + kvh) * kPartial<D, R>;
+  const uint64_t step = static_cast<uint64_t>(s.row_tiles) * a.pool.kv_heads * kPartial<D, R>;
+  const float *part = a.partial + (static_cast<uint64_t>(place.first + row / (32u * R)) * a.pool.kv_heads + kvh) * kPartial<D, R>;
   const float *ms = part + 32u * R * D + 2u * in, *os = part + in * D + lane * kPer;
   const float ninf = -__builtin_inff();
   float top = ninf;
