@@ -115,7 +115,8 @@ int launch(xpu_runtime *rt, const std::string &kernel, uint64_t grid, const A &a
 
 const char *type_name(int32_t dtype) { return dtype == XPU_DTYPE_FP16 ? "fp16" : "bf16"; }
 
-// How a tree attention call is cut (kernels/tree_attention.hip).
+// How a tree attention call is cut (kernels/tree_attention.hip). Every rule
+// goes by what the host knows: numbers of rows and sequences, not lengths.
 struct TreePlan {
   uint32_t sub_tiles = 1;  // of 32 rows per block
   uint32_t target = 1;     // chunks aimed at per kv head
@@ -127,8 +128,16 @@ struct TreePlan {
 TreePlan tree_plan(const xpu_runtime &rt, const xpu_cache &c, const xpu_batch &b, uint32_t heads) {
   TreePlan p;
   const uint64_t rows = static_cast<uint64_t>(b.rows) * (heads / c.kv_heads);
-  p.sub_tiles = rows > 32ull * b.n_seqs ? 2 : 1;
-  p.target = std::max(1u, 2 * rt.compute_units / c.kv_heads);
+  // 64 rows per block where sequences have more than 22 rows on average, so
+  // that the larger ones do not read their keys twice (48 ragged sequences of
+  // 1 .. 26 nodes x 4 heads, 28 rows on average, 98.4 us in 32s and 90.5 in
+  // 64s; 23 rows 93.8 and 90.5; 20 rows 86.8 and 88.2; 4 rows 69.5 and 72.7)
+  p.sub_tiles = rows > 22ull * b.n_seqs ? 2 : 1;
+  // a compute unit holds two blocks; ragged sequences balance better on three
+  // per unit, dealt as they end (48 drafts 96.3 -> 90.4 us, four long ones
+  // 472 -> 415), a single one is cut evenly (32000 positions 28.2 us at two,
+  // 31.7 at three)
+  p.target = std::max(1u, (b.n_seqs > 1 ? 3 : 2) * rt.compute_units / c.kv_heads);
   const uint64_t row_tiles = rows / (32 * p.sub_tiles) + b.n_seqs;
   const uint64_t tiles = (static_cast<uint64_t>(b.table_pitch) * c.page_size + 31) / 32;
   const bool cut = tiles > p.least;
@@ -136,6 +145,11 @@ TreePlan tree_plan(const xpu_runtime &rt, const xpu_cache &c, const xpu_batch &b
   p.bytes = cut ? p.slots * c.kv_heads * (32ull * p.sub_tiles * (c.head_dim + 2)) * 4 : 0;
   return p;
 }
+
+// Wavefronts that join a row's chunks: four for a few rows, whose chunks are
+// many (12 rows and heads of 256 chunks: 34.3 -> 28.5 us in all), one for
+// others (1536 of a few chunks: 75.8 us with four, 74.5 with one).
+constexpr uint64_t kWideJoins = 128;
 
 }  // namespace
 
@@ -216,7 +230,9 @@ int xpu_tree_attention(xpu_runtime *rt, const xpu_cache *cache, const xpu_batch 
                              "_r" + std::to_string(plan.sub_tiles);
     if (int rc = launch(rt, "xpu_tree_attention" + form, plan.slots * cache->kv_heads, a)) return rc;
     if (!plan.bytes) return XPU_OK;
-    return launch(rt, "xpu_tree_join" + form, (static_cast<uint64_t>(batch->rows) * heads + 3) / 4, a);
+    const uint64_t joins = static_cast<uint64_t>(batch->rows) * heads;
+    return joins <= kWideJoins ? launch(rt, "xpu_tree_join" + form + "_w4", joins, a)
+                               : launch(rt, "xpu_tree_join" + form, (joins + 3) / 4, a);
   });
 }
 
@@ -319,9 +335,12 @@ int xpu_prompt_attention(xpu_runtime *rt, const xpu_packed *p, const void *q, co
     a.heads = p->heads;
     a.kv_heads = p->kv_heads;
     a.scale_log2e = static_cast<float>(p->scale * kLog2e);
-    a.slots = p->q_rows / 128 + p->n_seqs;
+    // heads of a kv head that a block takes together, one or more wavefronts each
+    const uint32_t group = p->heads / p->kv_heads;
+    a.pack_shift = group % 4 == 0 ? 2 : group % 2 == 0 ? 1 : 0;
+    a.slots = p->q_rows / (128u >> a.pack_shift) + p->n_seqs;
     return launch(rt, std::string("xpu_packed_attention_") + type_name(p->dtype) + "_d" + std::to_string(p->head_dim),
-                  static_cast<uint64_t>(a.slots) * p->heads, a);
+                  static_cast<uint64_t>(a.slots) * (p->heads >> a.pack_shift), a);
   });
 }
 

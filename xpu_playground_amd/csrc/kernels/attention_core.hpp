@@ -92,13 +92,9 @@ template <int DT, int D, int R> struct Rows {
 #pragma unroll
     for (uint32_t ks = 0; ks < kKs; ++ks) q[r][ks] = *reinterpret_cast<const u32x4 *>(row + (2u * ks + hh) * 8u);
   }
-  // The same through LDS, for wavefronts that have their queries in common:
-  // 16 bytes per lane for each ks.
-  static constexpr uint32_t kQBytes = kKs * 1024u;  // of a sub-tile
-  XPU_DEVICE static void stage_q(uint32_t to, uint32_t ks, const uint16_t *row) {
-    *reinterpret_cast<lds_u32x4 *>(to + ks * 1024u + lane_id() * 16u) =
-        *reinterpret_cast<const u32x4 *>(row + (2u * ks + (lane_id() >> 5)) * 8u);
-  }
+  // A sub-tile's queries in LDS, for wavefronts that have them in common: 16
+  // bytes per lane for each ks.
+  static constexpr uint32_t kQBytes = kKs * 1024u;
 
   // S^T of sub-tile r and a tile of 32 T keys at LDS byte address kb; Q from
   // LDS at qb (QLDS) or from the registers. The reads run one step ahead of

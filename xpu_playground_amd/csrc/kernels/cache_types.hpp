@@ -18,7 +18,7 @@ struct PackedArgs {
   uint16_t *out;
   const uint32_t *q_starts, *k_starts;
   uint64_t q_stride, k_stride, v_stride, out_stride;  // elements
-  uint32_t n_seqs, q_rows, k_rows, heads, kv_heads, slots;
+  uint32_t n_seqs, q_rows, k_rows, heads, kv_heads, slots, pack_shift;
   float scale_log2e;
 };
 

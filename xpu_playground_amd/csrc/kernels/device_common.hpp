@@ -228,6 +228,14 @@ XPU_DEVICE void dma16(uint32_t m0, const i32x4 &r, uint32_t voff) {
                : "memory");
 }
 
+// The same for data that is read once: it does not stay in the L2.
+XPU_DEVICE void dma16_nt(uint32_t m0, const i32x4 &r, uint32_t voff) {
+  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen nt lds"
+               :
+               : "v"(voff), "s"(r), "{m0}"(m0)
+               : "memory");
+}
+
 template <int N> XPU_DEVICE void wait_vmcnt() {
   static_assert(N >= 0 && N < 64, "vmcnt is 6 bits");
   // gfx9 s_waitcnt: vmcnt[3:0] bits 3:0, vmcnt[5:4] bits 15:14; expcnt and

@@ -3,9 +3,11 @@
 // k_starts[s + 1] - 1; query i sees key j when j <= i + (keys - queries).
 // Row layout: [row][head][D], rows `stride` elements apart.
 //
-// Block: one query head, 4 wavefronts of 32 R queries each (QT = 128 R); key
-// tiles of 64 are staged by LDS-DMA, two stages of K then V, shared by the
-// wavefronts.
+// Block: 4 wavefronts of 32 queries; P = 1, 2 or 4 query heads of one kv head
+// (the group's largest such divisor) x 4 / P sub-tiles of the same sequence,
+// so that a sequence is cut into tiles of 128 / P queries: little is lost at
+// the ends of short sequences and at the diagonal. Key tiles of 64 are staged
+// by LDS-DMA, two stages of K then V, shared by the wavefronts.
 #include "attention_core.hpp"
 #include "cache_types.hpp"
 
@@ -13,20 +15,20 @@ namespace xpu {
 namespace att {
 
 // The sequence that owns slot `slot` of the work list, where sequence s has
-// the slots from starts[s] / tile + s on: at least as many as it has tiles,
-// and known without a sum over the sequences. -1: none.
-XPU_DEVICE int32_t sequence_of_slot(const uint32_t *starts, uint32_t n_seqs, uint32_t tile, uint32_t slot) {
+// the slots from starts[s] / tile + s on (tile = 1 << shift queries): at least
+// as many as it has tiles, and known without a sum over the sequences. -1: none.
+XPU_DEVICE int32_t sequence_of_slot(const uint32_t *starts, uint32_t n_seqs, uint32_t shift, uint32_t slot) {
   int32_t s = -1;
   for (uint32_t at = 0; at < n_seqs; at += 64) {
     const uint32_t i = at + lane_id();
-    const bool before = i < n_seqs && starts[i] / tile + i <= slot;
+    const bool before = i < n_seqs && (starts[i] >> shift) + i <= slot;
     s += __builtin_popcountll(__builtin_amdgcn_ballot_w64(before));
   }
   return __builtin_amdgcn_readfirstlane(s);
 }
 
-template <int DT, int D, int R> XPU_DEVICE void packed_attention(const PackedArgs &a) {
-  constexpr uint32_t kQt = 128u * R, kKeys = 64, kTile = kKeys * 2u * D, kStage = 2u * kTile;
+template <int DT, int D> XPU_DEVICE void packed_attention(const PackedArgs &a) {
+  constexpr uint32_t kKeys = 64, kTile = kKeys * 2u * D, kStage = 2u * kTile;
   constexpr uint32_t kRpi = 512u / D;          // key rows per DMA instruction
   constexpr uint32_t kCpr = D / 8;             // 16-byte chunks per key row
   constexpr uint32_t kDma = kKeys / kRpi / 4;  // DMA instructions per wave, K and V each
@@ -39,42 +41,42 @@ template <int DT, int D, int R> XPU_DEVICE void packed_attention(const PackedArg
   // Blocks are dealt to the 8 XCDs in turn: a kv head stays on one XCD (its K
   // and V in that L2) where the head count allows; within it the last slots,
   // the heaviest tiles of a sequence, come first.
-  const uint32_t group = a.heads / a.kv_heads;
+  const uint32_t group = a.heads / a.kv_heads, packs = group >> a.pack_shift;
   uint32_t kvh, rest;
   if (a.kv_heads % 8u == 0) {
     const uint32_t n = blockIdx.x / 8u;
-    kvh = blockIdx.x % 8u + 8u * (n / (a.slots * group));
-    rest = n % (a.slots * group);
+    kvh = blockIdx.x % 8u + 8u * (n / (a.slots * packs));
+    rest = n % (a.slots * packs);
   } else {
     kvh = blockIdx.x % a.kv_heads;
     rest = blockIdx.x / a.kv_heads;
   }
-  const uint32_t head = kvh * group + rest % group, slot = a.slots - 1u - rest / group;
+  const uint32_t slot = a.slots - 1u - rest / packs, qt_shift = 7u - a.pack_shift, q_tile = 1u << qt_shift;
+  const uint32_t head = kvh * group + (rest % packs << a.pack_shift) + (wave & (1u << a.pack_shift) - 1u);
 
-  const int32_t seq = sequence_of_slot(a.q_starts, a.n_seqs, kQt, slot);
+  const int32_t seq = sequence_of_slot(a.q_starts, a.n_seqs, qt_shift, slot);
   if (seq < 0) return;
   const uint32_t q_lo = __builtin_amdgcn_readfirstlane(a.q_starts[seq]);
   const uint32_t q_hi = __builtin_amdgcn_readfirstlane(a.q_starts[seq + 1]);
   const uint32_t k_lo = __builtin_amdgcn_readfirstlane(a.k_starts[seq]);
   const uint32_t k_hi = __builtin_amdgcn_readfirstlane(a.k_starts[seq + 1]);
   // starts that do not ascend or pass the rows: nothing of the sequence is touched
-  if (q_lo > q_hi || q_hi > a.q_rows || k_lo > k_hi || k_hi > a.k_rows || q_lo / kQt + seq > slot) return;
-  const uint32_t tile_q = slot - (q_lo / kQt + seq), n_q = q_hi - q_lo, n_k = k_hi - k_lo;
-  if (tile_q >= (n_q + kQt - 1) / kQt) return;
+  if (q_lo > q_hi || q_hi > a.q_rows || k_lo > k_hi || k_hi > a.k_rows || (q_lo >> qt_shift) + seq > slot) return;
+  const uint32_t first_q = (slot - ((q_lo >> qt_shift) + seq)) << qt_shift, n_q = q_hi - q_lo, n_k = k_hi - k_lo;
+  if (first_q >= n_q) return;
   const int32_t shift = static_cast<int32_t>(n_k) - static_cast<int32_t>(n_q);
-  const uint32_t t0 = tile_q * kQt + wave * 32u * R;  // the wave's first query
+  const uint32_t t0 = first_q + 32u * (wave >> a.pack_shift);  // the wave's first query
   // keys of the block and of the wave: 0 .. seen - 1
-  const int32_t block_seen = static_cast<int32_t>(min(tile_q * kQt + kQt, n_q)) + shift;
+  const int32_t block_seen = static_cast<int32_t>(min(first_q + q_tile, n_q)) + shift;
   const uint32_t n_seen = block_seen < 0 ? 0u : static_cast<uint32_t>(block_seen);
   const uint32_t n_tiles = (n_seen + kKeys - 1) / kKeys;
-  const int32_t wave_seen = static_cast<int32_t>(min(t0 + 32u * R, n_q)) + shift;
+  const int32_t wave_seen = static_cast<int32_t>(min(t0 + 32u, n_q)) + shift;
   const uint32_t wave_tiles = t0 < n_q && wave_seen > 0 ? (wave_seen + kKeys - 1) / kKeys : 0u;
 
-  Rows<DT, D, R> rows;
+  const uint32_t t = t0 + (lane & 31u);  // the lane's query
+  Rows<DT, D, 1> rows;
   rows.init();
-#pragma unroll
-  for (int r = 0; r < R; ++r)
-    rows.load_q(r, a.q + (q_lo + min(t0 + 32u * r + (lane & 31u), n_q - 1u)) * a.q_stride + head * D);
+  rows.load_q(0, a.q + (q_lo + min(t, n_q - 1u)) * a.q_stride + head * D);
 
   // DMA of the wave's share of a tile: instruction j fills LDS rows kRpi
   // (kDma wave + j) .., lane -> physical chunk lane % kCpr of row lane / kCpr.
@@ -105,7 +107,7 @@ template <int DT, int D, int R> XPU_DEVICE void packed_attention(const PackedArg
   for (uint32_t tile = 0; tile < n_tiles; ++tile) {
     const uint32_t stage = tile & 1u, kb = lds0 + stage * kStage, vb = kb + kTile;
     // whether some query of the block does not see some key of the tile
-    const bool edge = static_cast<int32_t>(tile * kKeys + kKeys - 1u) > static_cast<int32_t>(tile_q * kQt) + shift;
+    const bool edge = static_cast<int32_t>(tile * kKeys + kKeys - 1u) > static_cast<int32_t>(first_q) + shift;
     wait_vmcnt<0>();
     if (edge) {  // the V rows that this wave staged, before the barrier that publishes them
       bool bad = false;
@@ -120,58 +122,44 @@ template <int DT, int D, int R> XPU_DEVICE void packed_attention(const PackedArg
     __syncthreads();
     if (tile + 1 < n_tiles) issue(tile + 1, stage ^ 1u);
     const bool mine = tile < wave_tiles;
-    u32x8 pk[R][2];
-    uint32_t seen[R][2];
+    u32x8 pk[1][2];
+    uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
     if (mine) {
-      const bool masked = static_cast<int32_t>(tile * kKeys + kKeys - 1u) > static_cast<int32_t>(t0) + shift;
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        f32x16 s[2];
-        rows.template scores<2, false>(r, kb, 0, s);
-        seen[r][0] = seen[r][1] = 0xffffffffu;
-        if (masked) {  // wave-uniform
-          const int32_t last =
-              static_cast<int32_t>(t0 + 32u * r + (lane & 31u)) + shift - static_cast<int32_t>(tile * kKeys);
-          seen[r][0] = mask_to(last);
-          seen[r][1] = mask_to(last - 32);
-          Rows<DT, D, R>::template mask<2>(s, seen[r]);
-        }
-        rows.template softmax<2>(r, s, a.scale_log2e, pk[r]);
+      f32x16 s[2];
+      rows.template scores<2, false>(0, kb, 0, s);
+      if (static_cast<int32_t>(tile * kKeys + kKeys - 1u) > static_cast<int32_t>(t0) + shift) {  // wave-uniform
+        const int32_t last = static_cast<int32_t>(t) + shift - static_cast<int32_t>(tile * kKeys);
+        seen[0] = mask_to(last);
+        seen[1] = mask_to(last - 32);
+        Rows<DT, D, 1>::template mask<2>(s, seen);
       }
+      rows.template softmax<2>(0, s, a.scale_log2e, pk[0]);
     }
     if (edge && __builtin_expect(flags[stage][0] | flags[stage][1] | flags[stage][2] | flags[stage][3], 0)) {
       // the same in every wavefront: all read the rows before any clears its own
       if (mine) {
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          rows.add_apart(vb, r, pk[r][0], seen[r][0]);
-          rows.add_apart(vb + kTile / 2u, r, pk[r][1], seen[r][1]);
-        }
+        rows.add_apart(vb, 0, pk[0][0], seen[0]);
+        rows.add_apart(vb + kTile / 2u, 0, pk[0][1], seen[1]);
       }
       __syncthreads();
-      Rows<DT, D, R>::clear_apart(vb + wave * kTile / 4u, kKeys / 4u);
+      Rows<DT, D, 1>::clear_apart(vb + wave * kTile / 4u, kKeys / 4u);
       __syncthreads();
     }
     if (mine) rows.template values<2>(vb, pk);
   }
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const uint32_t t = t0 + 32u * r + (lane & 31u);
-    const float total = rows.total(r);
-    if (t < n_q)  // a query that sees no key: 0
-      rows.store(r, a.out + (q_lo + t) * a.out_stride + head * D,
-                 static_cast<int32_t>(t) + shift < 0 ? 0.0f : 1.0f / total);
-  }
+  const float total = rows.total(0);
+  if (t < n_q)  // a query that sees no key: 0
+    rows.store(0, a.out + (q_lo + t) * a.out_stride + head * D, static_cast<int32_t>(t) + shift < 0 ? 0.0f : 1.0f / total);
 }
 
 }  // namespace att
 }  // namespace xpu
 
-#define XPU_PACKED_ATTENTION(T, NAME, D, R)                                               \
-  extern "C" __global__ __launch_bounds__(256, 3 - R) void xpu_packed_attention_##NAME(xpu::PackedArgs a) { \
-    xpu::att::packed_attention<xpu::T, D, R>(a);                                          \
+#define XPU_PACKED_ATTENTION(T, NAME, D)                                                                  \
+  extern "C" __global__ __launch_bounds__(256, 2) void xpu_packed_attention_##NAME(xpu::PackedArgs a) {   \
+    xpu::att::packed_attention<xpu::T, D>(a);                                                             \
   }
-XPU_PACKED_ATTENTION(kBf16, bf16_d128, 128, 1)
-XPU_PACKED_ATTENTION(kFp16, fp16_d128, 128, 1)
-XPU_PACKED_ATTENTION(kBf16, bf16_d64, 64, 1)
-XPU_PACKED_ATTENTION(kFp16, fp16_d64, 64, 1)
+XPU_PACKED_ATTENTION(kBf16, bf16_d128, 128)
+XPU_PACKED_ATTENTION(kFp16, fp16_d128, 128)
+XPU_PACKED_ATTENTION(kBf16, bf16_d64, 64)
+XPU_PACKED_ATTENTION(kFp16, fp16_d64, 64)

@@ -20,6 +20,8 @@
 #include "attention_core.hpp"
 #include "cache_types.hpp"
 
+#include <type_traits>
+
 namespace xpu {
 namespace att {
 
@@ -47,59 +49,69 @@ XPU_DEVICE Sequence uniform_sequence(const BatchArgs &b, uint32_t page_size, uin
   return s;
 }
 
-XPU_DEVICE uint64_t wave_sum(uint64_t v) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+// Sums of lanes 0 .. own, with DPP moves: shifts within rows of 16 lanes, then
+// the rows' last lanes broadcast to the rows behind them.
+XPU_DEVICE uint32_t sum_upto(uint32_t v) {
+  auto add = [&](auto ctrl, auto rows) {
+    v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), ctrl.value, rows.value, 0xf, false));
+  };
+  using std::integral_constant;
+  constexpr integral_constant<int, 0xf> all;
+  add(integral_constant<int, 0x111>{}, all);  // row_shr:1, 2, 4, 8
+  add(integral_constant<int, 0x112>{}, all);
+  add(integral_constant<int, 0x114>{}, all);
+  add(integral_constant<int, 0x118>{}, all);
+  add(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});  // row_bcast:15 to rows 1 and 3
+  add(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});  // row_bcast:31 to rows 2 and 3
   return v;
 }
+XPU_DEVICE uint32_t wave_total(uint32_t v) { return __builtin_amdgcn_readlane(sum_upto(v), 63); }
 
 // How the keys are cut: every chunk has at most `most` tiles, so that the
 // chunks of all sequences and row tiles are at most target + the row tiles.
-template <int R> XPU_DEVICE uint32_t chunk_limit(const TreeArgs &a, uint32_t group) {
-  uint64_t work = 0;
-  for (uint32_t i = lane_id(); i < a.batch.n_seqs; i += 64) {
-    const Sequence s = sequence<R>(a.batch, a.pool.page_size, group, i);
-    work += static_cast<uint64_t>(s.row_tiles) * s.tiles;
-  }
-  work = wave_sum(work);
-  const uint64_t most = (work + a.target - 1) / a.target;
-  return __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(most < a.least ? a.least : most));
-}
-
 // The work items are numbered sequence by sequence, chunk by chunk, and row
 // tile by row tile within it, so that the row tiles that read the same keys
-// run side by side (and, with 8 kv heads, on one XCD). find() gives the sequence for which `is(first,
-// count, s)` holds, where first .. first + count - 1 are its items.
+// run side by side (and, with 8 kv heads, on one XCD). find() gives the
+// sequence for which `is(first, count, s)` holds, where first .. first + count
+// - 1 are its items. Every wavefront works this out by itself, a lane per
+// sequence, 64 sequences at a time.
 struct Place {
   int32_t seq;  // -1: none
   uint32_t first, chunks;
 };
-template <int R, typename Is> XPU_DEVICE Place find(const TreeArgs &a, uint32_t group, uint32_t most, Is &&is) {
-  uint32_t before = 0;
-  for (uint32_t at = 0; at < a.batch.n_seqs; at += 64) {
-    const uint32_t i = at + lane_id();
+template <int R, typename Is> XPU_DEVICE Place find(const TreeArgs &a, uint32_t group, Is &&is) {
+  const uint32_t n = a.batch.n_seqs;
+  auto of_lane = [&](uint32_t at) {
     Sequence s{};
-    uint32_t chunks = 0;
-    if (i < a.batch.n_seqs) {
-      s = sequence<R>(a.batch, a.pool.page_size, group, i);
-      chunks = (s.tiles + most - 1) / most;
-    }
-    const uint32_t count = s.row_tiles * chunks;
-    uint32_t upto = count;
-#pragma unroll
-    for (uint32_t d = 1; d < 64; d <<= 1) {
-      const uint32_t v = __shfl_up(upto, d);
-      if (lane_id() >= d) upto += v;
-    }
-    const uint32_t first = before + upto - count;
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(i < a.batch.n_seqs && is(first, count, s));
+    if (at + lane_id() < n) s = sequence<R>(a.batch, a.pool.page_size, group, at + lane_id());
+    return s;
+  };
+  Sequence s = of_lane(0);
+  uint64_t work = 0;
+  for (uint32_t at = 0;;) {
+    // 64 products of up to 2^50 in two sums of 32 bits
+    const uint64_t w = static_cast<uint64_t>(s.row_tiles) * s.tiles;
+    work += wave_total(static_cast<uint32_t>(w) & 0xffffffu) +
+            (static_cast<uint64_t>(wave_total(static_cast<uint32_t>(w >> 24))) << 24);
+    if ((at += 64) >= n) break;
+    s = of_lane(at);
+  }
+  const uint64_t share = (work + a.target - 1) / a.target;
+  const uint32_t most = share < a.least ? a.least : static_cast<uint32_t>(share);
+  uint32_t before = 0;
+  if (n > 64) s = of_lane(0);
+  for (uint32_t at = 0;;) {
+    const uint32_t chunks = (s.tiles + most - 1) / most, count = s.row_tiles * chunks;
+    const uint32_t upto = sum_upto(count), first = before + upto - count;
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(at + lane_id() < n && is(first, count, s));
     if (hit) {
       const uint32_t l = __builtin_ctzll(hit);
-      return {static_cast<int32_t>(__builtin_amdgcn_readfirstlane(at + l)),
-              static_cast<uint32_t>(__builtin_amdgcn_readlane(first, l)),
+      return {static_cast<int32_t>(at + l), static_cast<uint32_t>(__builtin_amdgcn_readlane(first, l)),
               static_cast<uint32_t>(__builtin_amdgcn_readlane(chunks, l))};
     }
+    if ((at += 64) >= n) break;
     before += __builtin_amdgcn_readlane(upto, 63);
+    s = of_lane(at);
   }
   return {-1, 0, 0};
 }
@@ -112,9 +124,10 @@ template <int DT, int D, int R> XPU_DEVICE void tree_attention(const TreeArgs &a
   constexpr uint32_t kRow = 2u * D, kTile = kTreeKeys * kRow;
   constexpr uint32_t kRpi = 512u / D, kCpr = D / 8;
   constexpr uint32_t kDma = kTreeKeys / kRpi;  // DMA instructions per tile, K and V each
-  constexpr uint32_t kMerge = 64u * R * (D / 2u) * 4u;  // bytes of one wave's output columns
-  constexpr uint32_t kLds = 8u * kTile > 2u * kMerge ? 8u * kTile : 2u * kMerge;
-  __shared__ __align__(1024) uint8_t lds[kLds];  // per wave a K and a V tile; then the partial results
+  // per wavefront a K and a V tile; then the partial results, D / 2 columns of
+  // 64 floats each (as many bytes)
+  __shared__ __align__(1024) uint8_t lds[8u * kTile];
+  static_assert(8u * kTile == 4u * 64u * (D / 2u) * 4u, "the partial results fit the tiles' memory");
   // the block's queries, then the (max, sum) pairs that its wavefronts exchange
   __shared__ __align__(16) uint8_t shared_q[R * Rows<DT, D, R>::kQBytes];
 
@@ -122,8 +135,7 @@ template <int DT, int D, int R> XPU_DEVICE void tree_attention(const TreeArgs &a
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t kvh = blockIdx.x % a.pool.kv_heads, item = blockIdx.x / a.pool.kv_heads;
   const uint32_t group = a.heads / a.pool.kv_heads;
-  const uint32_t most = chunk_limit<R>(a, group);
-  const Place place = find<R>(a, group, most, [&](uint32_t first, uint32_t count, const Sequence &) {
+  const Place place = find<R>(a, group, [&](uint32_t first, uint32_t count, const Sequence &) {
     return item >= first && item - first < count;
   });
   if (place.seq < 0) return;
@@ -146,19 +158,22 @@ template <int DT, int D, int R> XPU_DEVICE void tree_attention(const TreeArgs &a
   uint32_t w_from = t_lo * kTreeKeys >> a.pool.page_shift;
   uint32_t ids = window(w_from), ids_next = window(w_from + 64u);
 
+  // the wave's share of the queries: D / 64 of the 16-byte columns of every
+  // row; on their way while the first tiles are asked for
   const uint32_t qb = __builtin_amdgcn_readfirstlane(lds_addr(shared_q));
   Rows<DT, D, R> rows;
   rows.init();
   uint32_t node[R];
   uint64_t sees[R];  // bit j: node j
+  u32x4 q_part[R][D / 64];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const uint32_t row = min(row_tile * 32u * R + 32u * r + (lane & 31u), s.n * group - 1u);
+    const uint32_t row = min(32u * (row_tile * R + r) + (lane & 31u), s.n * group - 1u);
     node[r] = row / group;
     const uint16_t *q_row = a.q + (s.first + node[r]) * a.q_stride + (kvh * group + row % group) * D;
 #pragma unroll
     for (uint32_t j = 0; j < D / 64; ++j)
-      Rows<DT, D, R>::stage_q(qb + r * Rows<DT, D, R>::kQBytes, wave * (D / 64u) + j, q_row);
+      q_part[r][j] = *reinterpret_cast<const u32x4 *>(q_row + (2u * (wave * (D / 64u) + j) + hh) * 8u);
     if (a.visible) {
       sees[r] = a.visible[s.first + node[r]];
       if (s.n < 64u) sees[r] &= (1ull << s.n) - 1ull;
@@ -173,7 +188,7 @@ template <int DT, int D, int R> XPU_DEVICE void tree_attention(const TreeArgs &a
     k_off[j] = row * kRow + 16u * ((lane % kCpr) ^ k_swz<D>(row));
     v_off[j] = row * kRow + 16u * ((lane % kCpr) ^ v_swz<D>(row));
   }
-  const uint32_t kb = __builtin_amdgcn_readfirstlane(lds_addr(lds)) + wave * 2u * kTile, vb = kb + kTile;
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(lds)) + wave * 2u * kTile;
   const uint64_t head_at = static_cast<uint64_t>(kvh) * a.pool.page_size * D;
   // A tile is two halves of 16 keys, each inside one page (pages are 16 keys
   // or more). The descriptor ends with the sequence, so what older sequences
@@ -201,39 +216,46 @@ template <int DT, int D, int R> XPU_DEVICE void tree_attention(const TreeArgs &a
       live[h] = n * kRow;
     }
   };
-  auto issue = [&](const uint16_t *pool, uint32_t to, const uint32_t (&off)[kDma / 2], const uint64_t (&at)[2],
-                   const uint32_t (&bytes)[2]) {
+  // Keys that only this block reads (of a kv head's rows) pass by the L2; with
+  // more row tiles it serves the others.
+  const bool once = s.row_tiles == 1;
+  auto issue = [&](const uint16_t *pool, uint32_t to, const uint32_t (&off)[kDma / 2]) {
 #pragma unroll
     for (uint32_t h = 0; h < 2; ++h) {
-      const i32x4 d = rsrc(pool + at[h], static_cast<int64_t>(bytes[h]));
+      const i32x4 d = rsrc(pool + from[h], static_cast<int64_t>(live[h]));
+      const uint32_t at = to + h * kTile / 2u;
+      if (once) {
 #pragma unroll
-      for (uint32_t j = 0; j < kDma / 2; ++j) dma16(to + (h * kDma / 2 + j) * 1024u, d, off[j]);
+        for (uint32_t j = 0; j < kDma / 2; ++j) dma16_nt(at + j * 1024u, d, off[j]);
+      } else {
+#pragma unroll
+        for (uint32_t j = 0; j < kDma / 2; ++j) dma16(at + j * 1024u, d, off[j]);
+      }
     }
   };
 
   if (t_lo < t_hi) {
     locate(t_lo);
-    issue(a.pool.k, kb, k_off, from, live);
-    issue(a.pool.v, vb, v_off, from, live);
+    issue(a.pool.k, lds0, k_off);
+    issue(a.pool.v, lds0 + kTile, v_off);
   }
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (uint32_t j = 0; j < D / 64; ++j)
+      *reinterpret_cast<lds_u32x4 *>(qb + r * Rows<DT, D, R>::kQBytes + (wave * (D / 64u) + j) * 1024u + lane * 16u) =
+          q_part[r][j];
   __syncthreads();  // the queries are there
-  for (uint32_t tile = t_lo; tile < t_hi; ++tile) {
-    const bool more = tile + 1u < t_hi;
-    wait_vmcnt<kDma>();  // K is there; V may be on its way
+  // scores and softmax of a tile: p of every sub-tile, and which keys its
+  // queries see where not all of them do (edge, wave-uniform)
+  auto scored = [&](uint32_t tile, uint32_t kb, bool edge, u32x8 (&pk)[R][1], uint32_t (&seen)[R][1], auto &&after) {
     const int32_t base = static_cast<int32_t>(s.context - tile * kTreeKeys);  // node 0 in the tile
-    const bool edge = (tile + 1u) * kTreeKeys > s.context;  // the tile holds nodes (or ends the sequence)
-    u32x8 pk[R][1];
-    uint32_t seen[R][1] = {};
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       f32x16 sc[1];
       rows.template scores<1, true>(r, kb, qb, sc);
-      if (r == R - 1 && more) {
-        locate(tile + 1u);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K is read
-        issue(a.pool.k, kb, k_off, from, live);
-      }
-      if (edge) {  // wave-uniform
+      if (r == R - 1) after();
+      if (edge) {
         if (!a.visible) seen[r][0] = mask_to(base + static_cast<int32_t>(node[r]));
         else if (base >= 0) seen[r][0] = static_cast<uint32_t>(sees[r] << base) | ((1u << base) - 1u);
         else seen[r][0] = base > -64 ? static_cast<uint32_t>(sees[r] >> -base) : 0u;
@@ -241,135 +263,187 @@ template <int DT, int D, int R> XPU_DEVICE void tree_attention(const TreeArgs &a
       }
       rows.template softmax<1>(r, sc, a.scale_log2e, pk[r]);
     }
+  };
+  auto any_nonfinite = [&](uint32_t vb) {
+    bool odd = false;
+#pragma unroll
+    for (uint32_t j = 0; j < kDma; ++j) {
+      const u32x4 w = *reinterpret_cast<const lds_u32x4 *>(vb + j * 1024u + lane * 16u);
+      odd |= nonfinite<DT>(w.x) || nonfinite<DT>(w.y) || nonfinite<DT>(w.z) || nonfinite<DT>(w.w);
+    }
+    return __builtin_amdgcn_ballot_w64(odd) != 0;
+  };
+  auto reads_done = [] { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
+  // whether a tile holds nodes (or ends the sequence)
+  auto at_edge = [&](uint32_t tile) { return (tile + 1u) * kTreeKeys > s.context; };
+
+  // One stage: K of the next tile goes out once the scores have read this
+  // one's, V once P V has, so 8 to 16 KiB per wavefront are always on their way.
+  for (uint32_t tile = t_lo; tile < t_hi; ++tile) {
+    const bool more = tile + 1u < t_hi, edge = at_edge(tile);
+    const uint32_t kb = lds0, vb = kb + kTile;
+    u32x8 pk[R][1];
+    uint32_t seen[R][1] = {};
+    wait_vmcnt<kDma>();  // K is there; V may be on its way
+    scored(tile, kb, edge, pk, seen, [&] {
+      if (!more) return;
+      locate(tile + 1u);
+      reads_done();
+      issue(a.pool.k, kb, k_off);
+    });
     if (more) wait_vmcnt<kDma>();
     else wait_vmcnt<0>();
-    if (edge) {
-      bool odd = false;
+    if (edge && __builtin_expect(any_nonfinite(vb), 0)) {
 #pragma unroll
-      for (uint32_t j = 0; j < kDma; ++j) {
-        const u32x4 w = *reinterpret_cast<const lds_u32x4 *>(vb + j * 1024u + lane * 16u);
-        odd |= nonfinite<DT>(w.x) || nonfinite<DT>(w.y) || nonfinite<DT>(w.z) || nonfinite<DT>(w.w);
-      }
-      if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd) != 0, 0)) {
-#pragma unroll
-        for (int r = 0; r < R; ++r) rows.add_apart(vb, r, pk[r][0], seen[r][0]);
-        Rows<DT, D, R>::clear_apart(vb, kTreeKeys);
-      }
+      for (int r = 0; r < R; ++r) rows.add_apart(vb, r, pk[r][0], seen[r][0]);
+      Rows<DT, D, R>::clear_apart(vb, kTreeKeys);
     }
     rows.template values<1>(vb, pk);
-    if (more) {
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V is read
-      issue(a.pool.v, vb, v_off, from, live);
-    }
+    reads_done();
+    if (more) issue(a.pool.v, vb, v_off);
   }
 
-  // Waves 2 and 3 hand their results to 0 and 1, and 1 to 0. Each wave's sum
-  // is first that of both half-waves; `bad` makes the rows NaN.
-  float sum[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) sum[r] = bad ? __builtin_nanf("") : rows.total(r);
+  // The wavefronts' results meet in LDS, a sub-tile at a time; each wavefront
+  // adds up a quarter of the columns (kMine registers of every lane's D / 2),
+  // in the order of the keys. A side without a finite score has only zeros or
+  // NaN in its sum, which stay. `bad` makes the rows NaN.
   if (bad && lane == 0 && a.pool.status) *a.pool.status = 1u;
+  constexpr uint32_t kMine = D / 8;
   float *po = reinterpret_cast<float *>(lds), *meet = reinterpret_cast<float *>(shared_q);
 #pragma unroll
-  for (uint32_t half = 2; half; half >>= 1) {
-    __syncthreads();
-    if (wave >= half && wave < 2u * half) {
-      const uint32_t w = wave - half;
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        meet[((w * R + r) * 2u) * 64u + lane] = rows.m[r];
-        meet[((w * R + r) * 2u + 1u) * 64u + lane] = sum[r];
-#pragma unroll
-        for (uint32_t dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-          for (uint32_t i = 0; i < 16; ++i)
-            po[((w * R + r) * (D / 2u) + dt * 16u + i) * 64u + lane] = rows.o[r][dt][i];
-      }
-    }
-    __syncthreads();
-    if (wave < half) {
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const float m2 = meet[((wave * R + r) * 2u) * 64u + lane], s2 = meet[((wave * R + r) * 2u + 1u) * 64u + lane];
-        const float now = fmaxf(rows.m[r], m2), ninf = -__builtin_inff();
-        const float x = rows.m[r] == ninf ? 0.0f : __builtin_amdgcn_exp2f((rows.m[r] - now) * a.scale_log2e);
-        const float y = m2 == ninf ? 0.0f : __builtin_amdgcn_exp2f((m2 - now) * a.scale_log2e);
-        // a side without a finite score has only zeros or NaN, which stay
-        sum[r] = (rows.m[r] == ninf ? sum[r] : sum[r] * x) + (m2 == ninf ? s2 : s2 * y);
-#pragma unroll
-        for (uint32_t dt = 0; dt < D / 32; ++dt) {
-          __builtin_amdgcn_sched_barrier(0);  // 16 reads at a time: all of them would need the registers of `o` again
-#pragma unroll
-          for (uint32_t i = 0; i < 16; ++i) {
-            const float o2 = po[((wave * R + r) * (D / 2u) + dt * 16u + i) * 64u + lane];
-            rows.o[r][dt][i] = __builtin_fmaf(rows.o[r][dt][i], x, o2 * y);
-          }
-        }
-        rows.m[r] = now;
-      }
-    }
-  }
-  if (wave) return;
-#pragma unroll
   for (int r = 0; r < R; ++r) {
+    __syncthreads();  // the tiles, the queries, the sub-tile before are read
+    meet[(wave * 2u) * 64u + lane] = rows.m[r];
+    meet[(wave * 2u + 1u) * 64u + lane] = bad ? __builtin_nanf("") : rows.total(r);
+#pragma unroll
+    for (uint32_t dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (uint32_t i = 0; i < 16; ++i) po[(wave * (D / 2u) + dt * 16u + i) * 64u + lane] = rows.o[r][dt][i];
+    __syncthreads();
+    const float ninf = -__builtin_inff();
+    float m[4], x[4], top = ninf, sum = 0.0f;
+#pragma unroll
+    for (uint32_t w = 0; w < 4; ++w) top = fmaxf(top, m[w] = meet[w * 128u + lane]);
+#pragma unroll
+    for (uint32_t w = 0; w < 4; ++w) {
+      const float side = meet[w * 128u + 64u + lane];
+      x[w] = m[w] == ninf ? 0.0f : __builtin_amdgcn_exp2f((m[w] - top) * a.scale_log2e);
+      sum += m[w] == ninf ? side : side * x[w];
+    }
+    float o[kMine];
+#pragma unroll
+    for (uint32_t i = 0; i < kMine; ++i) {
+      o[i] = 0.0f;
+#pragma unroll
+      for (uint32_t w = 0; w < 4; ++w)
+        o[i] = __builtin_fmaf(po[(w * (D / 2u) + wave * kMine + i) * 64u + lane], x[w], o[i]);
+    }
+    // register wave * kMine + i: dims 32 (reg / 16) + 8 (reg % 16 / 4) + 4 hh + reg % 4
     const uint32_t in = 32u * r + (lane & 31u), row = row_tile * 32u * R + in;
+    const uint32_t dim = wave * 2u * kMine + 4u * hh;
     if (in >= rows_in) continue;
     if (place.chunks == 1) {
       const bool empty = s.context == 0 && a.visible && sees[r] == 0 && !bad;
-      rows.store(r, a.out + (s.first + row / group) * a.out_stride + (kvh * group + row % group) * D,
-                 empty ? 0.0f : 1.0f / sum[r]);
+      const float by = empty ? 0.0f : 1.0f / sum;
+      uint16_t *to = a.out + (s.first + row / group) * a.out_stride + (kvh * group + row % group) * D + dim;
+#pragma unroll
+      for (uint32_t w = 0; w < kMine / 4; ++w)
+        *reinterpret_cast<u32x2 *>(to + 8u * w) = u32x2{dma::cvt_pack<DT>(o[4 * w] * by, o[4 * w + 1] * by),
+                                                        dma::cvt_pack<DT>(o[4 * w + 2] * by, o[4 * w + 3] * by)};
     } else {
-      float *part = a.partial + (static_cast<uint64_t>(item) * a.pool.kv_heads + kvh) * kPartial<D, R>;
-      float *to = part + in * D + 4u * hh;
+      float *slot = a.partial + (static_cast<uint64_t>(item) * a.pool.kv_heads + kvh) * kPartial<D, R>;
+      float *to = slot + in * D + dim;
 #pragma unroll
-      for (uint32_t dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-        for (uint32_t w = 0; w < 4; ++w)
-          *reinterpret_cast<dma::f32x4 *>(to + 32u * dt + 8u * w) = dma::f32x4{
-              rows.o[r][dt][4 * w], rows.o[r][dt][4 * w + 1], rows.o[r][dt][4 * w + 2], rows.o[r][dt][4 * w + 3]};
-      if (hh == 0) {
-        part[32u * R * D + 2u * in] = rows.m[r];
-        part[32u * R * D + 2u * in + 1u] = sum[r];
-      }
+      for (uint32_t w = 0; w < kMine / 4; ++w)
+        *reinterpret_cast<dma::f32x4 *>(to + 8u * w) = dma::f32x4{o[4 * w], o[4 * w + 1], o[4 * w + 2], o[4 * w + 3]};
+      if (wave == 0 && hh == 0)
+        *reinterpret_cast<dma::f32x2 *>(slot + 32u * R * D + 2u * in) = dma::f32x2{top, sum};
     }
   }
 }
 
-// Adds the chunks of the rows whose keys were cut: one wavefront per (row,
-// query head), D / 64 output dims per lane, chunks in order.
-template <int DT, int D, int R> XPU_DEVICE void tree_join(const TreeArgs &a) {
-  constexpr uint32_t kPer = D / 64;
-  const uint32_t lane = lane_id(), index = blockIdx.x * 4u + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+// Adds the chunks of the rows whose keys were cut: W wavefronts per (row,
+// query head), each a W-th of the chunks. A lane takes one chunk's (max, sum)
+// of 64, then the half-waves every other chunk's outputs, D / 32 dims per
+// lane, kAhead loads in flight; the first of them go out with the (max, sum)
+// pairs, so that up to 2 kAhead chunks take one round trip to memory.
+template <int DT, int D, int R, int W> XPU_DEVICE void tree_join(const TreeArgs &a) {
+  constexpr uint32_t kPer = D / 32, kAhead = 8;
+  typedef float out_t __attribute__((ext_vector_type(kPer)));
+  const uint32_t lane = lane_id(), half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t index = W == 4 ? blockIdx.x : blockIdx.x * 4u + wave;
   const uint32_t row_at = index / a.heads, head = index % a.heads, group = a.heads / a.pool.kv_heads;
   if (row_at >= a.batch.rows) return;
-  const uint32_t most = chunk_limit<R>(a, group);
-  const Place place = find<R>(a, group, most, [&](uint32_t, uint32_t, const Sequence &s) {
+  const Place place = find<R>(a, group, [&](uint32_t, uint32_t, const Sequence &s) {
     return row_at >= s.first && row_at - s.first < s.n;
   });
   if (place.seq < 0 || place.chunks < 2) return;
   const Sequence s = uniform_sequence<R>(a.batch, a.pool.page_size, group, static_cast<uint32_t>(place.seq));
   const uint32_t kvh = head / group, row = (row_at - s.first) * group + head % group;
   const uint32_t in = row % (32u * R);
+  const uint32_t begin = W == 4 ? place.chunks * wave / 4u : 0u, chunks = W == 4 ? place.chunks * (wave + 1u) / 4u : place.chunks;
   const uint64_t step = static_cast<uint64_t>(s.row_tiles) * a.pool.kv_heads * kPartial<D, R>;
   const float *part = a.partial + (static_cast<uint64_t>(place.first + row / (32u * R)) * a.pool.kv_heads + kvh) * kPartial<D, R>;
-  const float *ms = part + 32u * R * D + 2u * in, *os = part + in * D + lane * kPer;
+  const float *ms = part + 32u * R * D + 2u * in, *os = part + in * D + (lane & 31u) * kPer;
   const float ninf = -__builtin_inff();
-  float top = ninf;
-  for (uint32_t c = lane; c < place.chunks; c += 64) top = fmaxf(top, ms[c * step]);
-  top = wave_reduce(top, [](float x, float y) { return fmaxf(x, y); });
-  float sum = 0.0f, o[kPer] = {};
-#pragma unroll 4
-  for (uint32_t c = 0; c < place.chunks; ++c) {
-    const float m = ms[c * step], l = ms[c * step + 1];
-    const float x = m == ninf ? 0.0f : __builtin_amdgcn_exp2f((m - top) * a.scale_log2e);
-    sum += m == ninf ? l : l * x;  // no finite score: zeros or NaN
+  float top = ninf, sum = 0.0f;
+  out_t o = {}, v[kAhead];
+  auto ask = [&](uint32_t c) {  // past the last chunk: it again, with weight 0
 #pragma unroll
-    for (uint32_t i = 0; i < kPer; ++i) o[i] = __builtin_fmaf(os[c * step + i], x, o[i]);
+    for (uint32_t i = 0; i < kAhead; ++i)
+      v[i] = *reinterpret_cast<const out_t *>(os + min(c + 2u * i + half, chunks - 1u) * step);
+  };
+  for (uint32_t c0 = begin; c0 < chunks; c0 += 64) {
+    const uint32_t mine = c0 + lane;
+    const dma::f32x2 ml = *reinterpret_cast<const dma::f32x2 *>(ms + min(mine, chunks - 1u) * step);
+    ask(c0);
+    const float m = mine < chunks ? ml.x : ninf, l = mine < chunks ? ml.y : 0.0f;
+    const float now = fmaxf(top, wave_reduce(m, [](float x, float y) { return fmaxf(x, y); }));
+    const float old = top == ninf ? 0.0f : __builtin_amdgcn_exp2f((top - now) * a.scale_log2e);
+    const float x = m == ninf ? 0.0f : __builtin_amdgcn_exp2f((m - now) * a.scale_log2e);
+    // without a finite score the sum is zeros or NaN, which stay
+    sum = (top == ninf ? sum : sum * old) + wave_butterfly(m == ninf ? l : l * x);
+    o *= old;
+    top = now;
+    const uint32_t n = min(chunks - c0, 64u);
+    for (uint32_t j = 0; j < n; j += 2u * kAhead) {
+      if (j) ask(c0 + j);
+#pragma unroll
+      for (uint32_t i = 0; i < kAhead; ++i) {
+        const float even = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), j + 2u * i));
+        const float odd = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), j + 2u * i + 1u));
+        const float w = half ? odd : even;
+#pragma unroll
+        for (uint32_t d = 0; d < kPer; ++d) o[d] = __builtin_fmaf(v[i][d], w, o[d]);
+      }
+    }
+  }
+  if constexpr (W == 4) {
+    __shared__ float tops[4], sums[4];
+    __shared__ __align__(16) out_t outs[4][64];
+    if (lane == 0) tops[wave] = top, sums[wave] = sum;
+    outs[wave][lane] = o;
+    __syncthreads();
+    if (wave) return;
+    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    sum = 0.0f;
+    o = 0.0f;
+#pragma unroll
+    for (uint32_t w = 0; w < 4; ++w) {
+      const float x = tops[w] == ninf ? 0.0f : __builtin_amdgcn_exp2f((tops[w] - top) * a.scale_log2e);
+      sum += tops[w] == ninf ? sums[w] : sums[w] * x;
+      o += outs[w][lane] * x;
+    }
   }
   const float by = 1.0f / sum;  // a row that sees nothing has at most 64 positions, which are never cut
+#pragma unroll
+  for (uint32_t d = 0; d < kPer; ++d) o[d] = (o[d] + xor32_f(o[d])) * by;
+  if (half) return;
   uint16_t *to = a.out + row_at * a.out_stride + head * D + lane * kPer;
-  if constexpr (kPer == 2) *reinterpret_cast<uint32_t *>(to) = dma::cvt_pack<DT>(o[0] * by, o[1] * by);
-  else *to = static_cast<uint16_t>(dma::cvt_pack<DT>(o[0] * by, 0.0f));
+  if constexpr (kPer == 4)
+    *reinterpret_cast<u32x2 *>(to) = u32x2{dma::cvt_pack<DT>(o[0], o[1]), dma::cvt_pack<DT>(o[2], o[3])};
+  else
+    *reinterpret_cast<uint32_t *>(to) = dma::cvt_pack<DT>(o[0], o[1]);
 }
 
 }  // namespace att
@@ -380,7 +454,10 @@ template <int DT, int D, int R> XPU_DEVICE void tree_join(const TreeArgs &a) {
     xpu::att::tree_attention<xpu::T, D, R>(a);                                                            \
   }                                                                                                       \
   extern "C" __global__ __launch_bounds__(256) void xpu_tree_join_##NAME(xpu::TreeArgs a) {               \
-    xpu::att::tree_join<xpu::T, D, R>(a);                                                                 \
+    xpu::att::tree_join<xpu::T, D, R, 1>(a);                                                              \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(256) void xpu_tree_join_##NAME##_w4(xpu::TreeArgs a) {          \
+    xpu::att::tree_join<xpu::T, D, R, 4>(a);                                                              \
   }
 XPU_TREE_ATTENTION(kBf16, bf16_d128_r1, 128, 1)
 XPU_TREE_ATTENTION(kFp16, fp16_d128_r1, 128, 1)
