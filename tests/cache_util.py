@@ -8,15 +8,18 @@ sum_j p_j from p_j = 2^((s_j - m) log2 e), where
     (the MFMA may round each product and partial sum), and the exponent's
     argument |s_j - m| log2 e by that times 2^-23 more; with 2^-21 for exp2:
     a relative error e_j of p_j,
-  - p_j is rounded to the storage type for the product (u = half a step
-    relative), in fp16 with an absolute 2^-25 below its normal range; the sum
-    takes p_j unrounded, and sum p >= 1 in the same scale, since the reference
-    m is the score of some key,
+  - p_j is rounded to the storage type (u = half a step relative), in fp16 with
+    an absolute 2^-25 below its normal range, and the rounded values P_j are
+    what both sums take: sum P v / sum P - o = sum (P - p) (v - o) / sum P, where
+    sum P >= 1 in the scale of p, since the reference m is the score of some key
+    (p = 1); so it is at most u sum w |v - o| / (1 - u) <= u (sum w |v| + |o|) /
+    (1 - u), and in fp16 2^-25 (sum |v| + n |o|) more,
   - the FP32 sums of n terms are off by n 2^-23 relative to sum w |v|,
   - the result is rounded once (u).
-Hence |error| <= (u + 2 max e + n 2^-22) sum w |v| + 2^-25 sum |v| (fp16) +
-u |o|, and a subnormal result half its step more. Merging partial results adds
-a few 2^-22 per merge, counted with e.
+Hence |error| <= (u + 2 max e + n 2^-22) sum w |v| + u |o| + 2^-25 (sum |v| + n
+|o|) (fp16) + u |o|, all with a factor 1 + 3 u for the products of these, and a
+subnormal result half its step more. Merging partial results adds a few 2^-22
+per merge, counted with e.
 """
 import numpy as np
 import torch
@@ -95,9 +98,9 @@ def attend(q, k, v, seen, scale, dtype, merges=4):
             e = ((d + 2) * scale * (np.abs(k[at]) @ np.abs(q[i])).max() + np.abs(s - s.max()).max()) * 2.0 ** -23
             e += (2 + merges) * 2.0 ** -22
             out[i] = o
-            tol[i] = ((u + 2 * e + len(at) * 2.0 ** -22) * size + (2.0 ** -25 * total if dtype == xpu.FP16 else 0) +
-                      u * np.abs(o) + TINY[dtype])
-            tol[i] *= 1 + 2 * u
+            small = 2.0 ** -25 * (total + len(at) * np.abs(o)) if dtype == xpu.FP16 else 0
+            tol[i] = (u + 2 * e + len(at) * 2.0 ** -22) * size + 2 * u * np.abs(o) + small + TINY[dtype]
+            tol[i] *= 1 + 3 * u
     return out, tol
 
 

@@ -101,6 +101,22 @@ def test_ascending_scores(rt, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shift", [6.0, 10.4, 11.1, 13.9, 16.0])
+def test_many_small_probabilities(rt, dtype, shift):
+    """One key far above thousands of others, whose probabilities are in or
+    below the subnormal range of fp16 and together make a good part of the sum."""
+    n, d = 4000, 64
+    q, k = codes(np.ones((1, 1, d)), dtype), np.full((n, 1, d), -shift / d, np.float32)
+    k[1234] = 0
+    v = np.ones((n, 1, d), np.float32)
+    v[1234] = 0
+    k, v = codes(k, dtype), codes(v, dtype)
+    got = launch(rt, q, k, v, u32([0, 1]), u32([0, n]), dtype, 1.0)
+    want, tol = expected(q, k, v, u32([0, 1]), u32([0, n]), 1.0, dtype, np.zeros(q.shape, np.uint16))
+    check(values(got, dtype), want, tol)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("bad", ["nan", "inf"])
 @pytest.mark.parametrize("at", [5, 40, 63, 64, 131, 199])

@@ -54,6 +54,17 @@ template <int DT> XPU_DEVICE bool nonfinite(uint32_t w) {
   return (w & e) == e || (w & (e << 16)) == (e << 16);
 }
 
+// v + both 16-bit values of a word: one instruction for the two additions.
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+template <int DT> XPU_DEVICE float add_pair(uint32_t w, float v) {
+  if constexpr (DT == kFp16)
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), f16x2{1.0f, 1.0f}, v, false);
+  else
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), bf16x2{1.0f, 1.0f}, v, false);
+}
+
 // One wavefront's queries. R: sub-tiles of 32 rows.
 template <int DT, int D, int R> struct Rows {
   static_assert(D == 64 || D == 128, "head sizes");
@@ -62,9 +73,10 @@ template <int DT, int D, int R> struct Rows {
   u32x4 q[R][kKs];
   f32x16 o[R][kDt];
   float m[R], sum[R];
-  uint32_t ka[kKs], va[kDt];  // the lane's LDS offsets in a K and a V tile
+  uint32_t ka[kKs], va[kDt];  // the lane's LDS addresses in a K and a V tile at `base`
 
-  XPU_DEVICE void init() {
+  // base: the LDS address that the tiles' offsets (kb, vb below) count from
+  XPU_DEVICE void init(uint32_t base) {
     const uint32_t lane = lane_id(), hh = lane >> 5;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -77,13 +89,13 @@ template <int DT, int D, int R> struct Rows {
     }
     const uint32_t row = lane & 31u;
 #pragma unroll
-    for (uint32_t ks = 0; ks < kKs; ++ks) ka[ks] = row * kRow + 16u * ((2u * ks + hh) ^ k_swz<D>(row));
+    for (uint32_t ks = 0; ks < kKs; ++ks) ka[ks] = base + row * kRow + 16u * ((2u * ks + hh) ^ k_swz<D>(row));
     // the transposing read: lane i of a 16-lane group gives row (i % 16) / 4
     // of the group's 4 rows, dims 16 ((lane / 16) % 2) + 4 (lane % 4)
     const uint32_t tr_row = (lane & 15u) >> 2, tr_chunk = 2u * ((lane >> 4) & 1u) + ((lane & 3u) >> 1);
 #pragma unroll
     for (uint32_t dt = 0; dt < kDt; ++dt)
-      va[dt] = (4u * hh + tr_row) * kRow + 16u * ((4u * dt + tr_chunk) ^ v_swz<D>(tr_row)) + 8u * (lane & 1u);
+      va[dt] = base + (4u * hh + tr_row) * kRow + 16u * ((4u * dt + tr_chunk) ^ v_swz<D>(tr_row)) + 8u * (lane & 1u);
   }
 
   // Q row of sub-tile r: dims 16 ks + 8 hh .. + 7 in every ks
@@ -96,7 +108,7 @@ template <int DT, int D, int R> struct Rows {
   // bytes per lane for each ks.
   static constexpr uint32_t kQBytes = kKs * 1024u;
 
-  // S^T of sub-tile r and a tile of 32 T keys at LDS byte address kb; Q from
+  // S^T of sub-tile r and a tile of 32 T keys at LDS offset kb; Q from
   // LDS at qb (QLDS) or from the registers. The reads run one step ahead of
   // the MFMAs; the barriers keep the compiler from moving all of them to the
   // front, which would take more registers than there are.
@@ -174,14 +186,14 @@ template <int DT, int D, int R> struct Rows {
       for (int i = 0; i < 16; i += 2) {
         const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], c, shift));
         const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i + 1], c, shift));
-        part = part + e0 + e1;
         pk[t][i / 2] = dma::cvt_pack<DT>(e0, e1);
+        part = add_pair<DT>(pk[t][i / 2], part);
       }
     sum[r] += part;
   }
 
-  // O^T += V^T P^T for the tile at LDS byte address vb, the reads one step (16
-  // keys) ahead of the MFMAs.
+  // O^T += V^T P^T for the tile at LDS offset vb, the reads one step (16 keys)
+  // ahead of the MFMAs.
   template <int T> XPU_DEVICE void values(uint32_t vb, const u32x8 (&pk)[R][T]) {
     u32x4 vf[2][kDt];
     auto read = [&](uint32_t ks) {

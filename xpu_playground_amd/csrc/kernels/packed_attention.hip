@@ -11,6 +11,8 @@
 #include "attention_core.hpp"
 #include "cache_types.hpp"
 
+#include <type_traits>
+
 namespace xpu {
 namespace att {
 
@@ -74,8 +76,9 @@ template <int DT, int D> XPU_DEVICE void packed_attention(const PackedArgs &a) {
   const uint32_t wave_tiles = t0 < n_q && wave_seen > 0 ? (wave_seen + kKeys - 1) / kKeys : 0u;
 
   const uint32_t t = t0 + (lane & 31u);  // the lane's query
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(lds));
   Rows<DT, D, 1> rows;
-  rows.init();
+  rows.init(lds0);
   rows.load_q(0, a.q + (q_lo + min(t, n_q - 1u)) * a.q_stride + head * D);
 
   // DMA of the wave's share of a tile: instruction j fills LDS rows kRpi
@@ -88,7 +91,6 @@ template <int DT, int D> XPU_DEVICE void packed_attention(const PackedArgs &a) {
     k_off[j] = row * static_cast<uint32_t>(a.k_stride) * 2u + 16u * ((lane % kCpr) ^ k_swz<D>(row));
     v_off[j] = row * static_cast<uint32_t>(a.v_stride) * 2u + 16u * ((lane % kCpr) ^ v_swz<D>(row));
   }
-  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(lds));
   const uint16_t *k_head = a.k + static_cast<uint64_t>(k_lo) * a.k_stride + kvh * D;
   const uint16_t *v_head = a.v + static_cast<uint64_t>(k_lo) * a.v_stride + kvh * D;
   auto issue = [&](uint32_t tile, uint32_t stage) {
@@ -103,9 +105,10 @@ template <int DT, int D> XPU_DEVICE void packed_attention(const PackedArgs &a) {
     for (uint32_t j = 0; j < kDma; ++j) dma16(at + kTile + j * 1024u, rv, v_off[j]);
   };
 
-  if (n_tiles) issue(0, 0);
-  for (uint32_t tile = 0; tile < n_tiles; ++tile) {
-    const uint32_t stage = tile & 1u, kb = lds0 + stage * kStage, vb = kb + kTile;
+  // one tile of keys; the stage is a constant, so the LDS reads' addresses are
+  // registers and constant offsets
+  auto step = [&](uint32_t tile, auto stage_of) {
+    constexpr uint32_t stage = stage_of, kb = stage * kStage, vb = kb + kTile;
     // whether some query of the block does not see some key of the tile
     const bool edge = static_cast<int32_t>(tile * kKeys + kKeys - 1u) > static_cast<int32_t>(first_q) + shift;
     wait_vmcnt<0>();
@@ -113,7 +116,7 @@ template <int DT, int D> XPU_DEVICE void packed_attention(const PackedArgs &a) {
       bool bad = false;
 #pragma unroll
       for (uint32_t j = 0; j < kDma; ++j) {
-        const u32x4 w = *reinterpret_cast<const lds_u32x4 *>(vb + (wave * kDma + j) * 1024u + lane * 16u);
+        const u32x4 w = *reinterpret_cast<const lds_u32x4 *>(lds0 + vb + (wave * kDma + j) * 1024u + lane * 16u);
         bad |= nonfinite<DT>(w.x) || nonfinite<DT>(w.y) || nonfinite<DT>(w.z) || nonfinite<DT>(w.w);
       }
       const bool any = __builtin_amdgcn_ballot_w64(bad) != 0;
@@ -138,14 +141,19 @@ template <int DT, int D> XPU_DEVICE void packed_attention(const PackedArgs &a) {
     if (edge && __builtin_expect(flags[stage][0] | flags[stage][1] | flags[stage][2] | flags[stage][3], 0)) {
       // the same in every wavefront: all read the rows before any clears its own
       if (mine) {
-        rows.add_apart(vb, 0, pk[0][0], seen[0]);
-        rows.add_apart(vb + kTile / 2u, 0, pk[0][1], seen[1]);
+        rows.add_apart(lds0 + vb, 0, pk[0][0], seen[0]);
+        rows.add_apart(lds0 + vb + kTile / 2u, 0, pk[0][1], seen[1]);
       }
       __syncthreads();
-      Rows<DT, D, 1>::clear_apart(vb + wave * kTile / 4u, kKeys / 4u);
+      Rows<DT, D, 1>::clear_apart(lds0 + vb + wave * kTile / 4u, kKeys / 4u);
       __syncthreads();
     }
     if (mine) rows.template values<2>(vb, pk);
+  };
+  if (n_tiles) issue(0, 0);
+  for (uint32_t tile = 0; tile < n_tiles; tile += 2) {
+    step(tile, std::integral_constant<uint32_t, 0>{});
+    if (tile + 1 < n_tiles) step(tile + 1, std::integral_constant<uint32_t, 1>{});
   }
   const float total = rows.total(0);
   if (t < n_q)  // a query that sees no key: 0

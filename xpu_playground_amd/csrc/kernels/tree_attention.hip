@@ -162,7 +162,8 @@ template <int DT, int D, int R> XPU_DEVICE void tree_attention(const TreeArgs &a
   // row; on their way while the first tiles are asked for
   const uint32_t qb = __builtin_amdgcn_readfirstlane(lds_addr(shared_q));
   Rows<DT, D, R> rows;
-  rows.init();
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(lds)) + wave * 2u * kTile;
+  rows.init(lds0);
   uint32_t node[R];
   uint64_t sees[R];  // bit j: node j
   u32x4 q_part[R][D / 64];
@@ -188,7 +189,6 @@ template <int DT, int D, int R> XPU_DEVICE void tree_attention(const TreeArgs &a
     k_off[j] = row * kRow + 16u * ((lane % kCpr) ^ k_swz<D>(row));
     v_off[j] = row * kRow + 16u * ((lane % kCpr) ^ v_swz<D>(row));
   }
-  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(lds)) + wave * 2u * kTile;
   const uint64_t head_at = static_cast<uint64_t>(kvh) * a.pool.page_size * D;
   // A tile is two halves of 16 keys, each inside one page (pages are 16 keys
   // or more). The descriptor ends with the sequence, so what older sequences
@@ -248,12 +248,12 @@ template <int DT, int D, int R> XPU_DEVICE void tree_attention(const TreeArgs &a
   __syncthreads();  // the queries are there
   // scores and softmax of a tile: p of every sub-tile, and which keys its
   // queries see where not all of them do (edge, wave-uniform)
-  auto scored = [&](uint32_t tile, uint32_t kb, bool edge, u32x8 (&pk)[R][1], uint32_t (&seen)[R][1], auto &&after) {
+  auto scored = [&](uint32_t tile, bool edge, u32x8 (&pk)[R][1], uint32_t (&seen)[R][1], auto &&after) {
     const int32_t base = static_cast<int32_t>(s.context - tile * kTreeKeys);  // node 0 in the tile
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       f32x16 sc[1];
-      rows.template scores<1, true>(r, kb, qb, sc);
+      rows.template scores<1, true>(r, 0, qb, sc);
       if (r == R - 1) after();
       if (edge) {
         if (!a.visible) seen[r][0] = mask_to(base + static_cast<int32_t>(node[r]));
@@ -281,26 +281,25 @@ template <int DT, int D, int R> XPU_DEVICE void tree_attention(const TreeArgs &a
   // one's, V once P V has, so 8 to 16 KiB per wavefront are always on their way.
   for (uint32_t tile = t_lo; tile < t_hi; ++tile) {
     const bool more = tile + 1u < t_hi, edge = at_edge(tile);
-    const uint32_t kb = lds0, vb = kb + kTile;
     u32x8 pk[R][1];
     uint32_t seen[R][1] = {};
     wait_vmcnt<kDma>();  // K is there; V may be on its way
-    scored(tile, kb, edge, pk, seen, [&] {
+    scored(tile, edge, pk, seen, [&] {
       if (!more) return;
       locate(tile + 1u);
       reads_done();
-      issue(a.pool.k, kb, k_off);
+      issue(a.pool.k, lds0, k_off);
     });
     if (more) wait_vmcnt<kDma>();
     else wait_vmcnt<0>();
-    if (edge && __builtin_expect(any_nonfinite(vb), 0)) {
+    if (edge && __builtin_expect(any_nonfinite(lds0 + kTile), 0)) {
 #pragma unroll
-      for (int r = 0; r < R; ++r) rows.add_apart(vb, r, pk[r][0], seen[r][0]);
-      Rows<DT, D, R>::clear_apart(vb, kTreeKeys);
+      for (int r = 0; r < R; ++r) rows.add_apart(lds0 + kTile, r, pk[r][0], seen[r][0]);
+      Rows<DT, D, R>::clear_apart(lds0 + kTile, kTreeKeys);
     }
-    rows.template values<1>(vb, pk);
+    rows.template values<1>(kTile, pk);
     reads_done();
-    if (more) issue(a.pool.v, vb, v_off);
+    if (more) issue(a.pool.v, lds0 + kTile, v_off);
   }
 
   // The wavefronts' results meet in LDS, a sub-tile at a time; each wavefront
