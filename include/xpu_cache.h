@@ -102,7 +102,8 @@ int xpu_tree_attention_workspace(const xpu_runtime *rt, const xpu_cache *cache, 
 /* The accepted nodes of each sequence's rows move to the front, in all
  * layers: new position context[s] + j = what position context[s] + kept[
  * starts[s] + j] held before the call, for j < counts[s] (at most 64 and at
- * most the sequence's rows). kept may repeat nodes and be in any order. The
+ * most the sequence's rows). kept names nodes 0 .. 63 of the sequence's rows,
+ * in any order and more than once if need be. The
  * positions behind the kept ones hold what they held. new_context (NULL, or
  * n_seqs entries apart from context): context[s] + counts[s]. A sequence with
  * a count that does not fit is left alone, and so is a row with a node or a

@@ -252,8 +252,8 @@ int xpu_cache_keep(xpu_runtime *rt, const xpu_cache *cache, const xpu_batch *bat
       return invalid(name, "new_context must not overlap context, counts or starts");
     if (int rc = check_runtime(name, rt)) return rc;
     const xpu::KeepArgs a{pool_of(*cache), batch_of(*batch), kept, counts, new_context};
-    const uint64_t waves = static_cast<uint64_t>(batch->n_seqs) * cache->layers * cache->kv_heads * 2;
-    return launch(rt, cache->head_dim == 128 ? "xpu_cache_keep_d128" : "xpu_cache_keep_d64", (waves + 3) / 4, a);
+    const uint64_t groups = (static_cast<uint64_t>(cache->layers) * cache->kv_heads * 2 + 3) / 4;
+    return launch(rt, cache->head_dim == 128 ? "xpu_cache_keep_d128" : "xpu_cache_keep_d64", batch->n_seqs * groups, a);
   });
 }
 

@@ -24,6 +24,8 @@
 #pragma once
 #include "device_common.hpp"
 
+#include <type_traits>
+
 namespace xpu {
 namespace att {
 
@@ -65,6 +67,24 @@ template <int DT> XPU_DEVICE float add_pair(uint32_t w, float v) {
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), bf16x2{1.0f, 1.0f}, v, false);
 }
 
+// Sums of lanes 0 .. own, with DPP moves: shifts within rows of 16 lanes, then
+// the rows' last lanes broadcast to the rows behind them.
+XPU_DEVICE uint32_t sum_upto(uint32_t v) {
+  auto add = [&](auto ctrl, auto rows) {
+    v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), ctrl.value, rows.value, 0xf, false));
+  };
+  using std::integral_constant;
+  constexpr integral_constant<int, 0xf> all;
+  add(integral_constant<int, 0x111>{}, all);  // row_shr:1, 2, 4, 8
+  add(integral_constant<int, 0x112>{}, all);
+  add(integral_constant<int, 0x114>{}, all);
+  add(integral_constant<int, 0x118>{}, all);
+  add(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});  // row_bcast:15 to rows 1 and 3
+  add(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});  // row_bcast:31 to rows 2 and 3
+  return v;
+}
+XPU_DEVICE uint32_t wave_total(uint32_t v) { return __builtin_amdgcn_readlane(sum_upto(v), 63); }
+
 // One wavefront's queries. R: sub-tiles of 32 rows.
 template <int DT, int D, int R> struct Rows {
   static_assert(D == 64 || D == 128, "head sizes");
@@ -98,11 +118,11 @@ template <int DT, int D, int R> struct Rows {
       va[dt] = base + (4u * hh + tr_row) * kRow + 16u * ((4u * dt + tr_chunk) ^ v_swz<D>(tr_row)) + 8u * (lane & 1u);
   }
 
-  // Q row of sub-tile r: dims 16 ks + 8 hh .. + 7 in every ks
-  XPU_DEVICE void load_q(int r, const uint16_t *row) {
-    const uint32_t hh = lane_id() >> 5;
+  // The queries of sub-tile 0 from 32 rows at LDS offset `at`, laid out as a
+  // tile's K rows: dims 16 ks + 8 hh .. + 7 of the lane's query in every ks.
+  XPU_DEVICE void read_q(uint32_t at) {
 #pragma unroll
-    for (uint32_t ks = 0; ks < kKs; ++ks) q[r][ks] = *reinterpret_cast<const u32x4 *>(row + (2u * ks + hh) * 8u);
+    for (uint32_t ks = 0; ks < kKs; ++ks) q[0][ks] = *reinterpret_cast<const lds_u32x4 *>(ka[ks] + at);
   }
   // A sub-tile's queries in LDS, for wavefronts that have them in common: 16
   // bytes per lane for each ks.
@@ -157,16 +177,19 @@ template <int DT, int D, int R> struct Rows {
     }
   }
 
-  // The running maximum, and p of the tile packed as the MFMA takes it:
-  // word i of pk[t] holds registers 2 i and 2 i + 1. c = scale log2 e > 0.
-  template <int T> XPU_DEVICE void softmax(int r, const f32x16 (&s)[T], float c, u32x8 (&pk)[T]) {
-    const float ninf = -__builtin_inff();
-    float top = ninf;
+  // The largest score of each query.
+  template <int T> XPU_DEVICE static float largest(const f32x16 (&s)[T]) {
+    float top = -__builtin_inff();
 #pragma unroll
     for (int t = 0; t < T; ++t)
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
-    top = fmaxf(top, xor32_f(top));  // the query's other half-wave
+    return fmaxf(top, xor32_f(top));  // the query's other half-wave
+  }
+  // Moves the reference where `top` passes it by more than kLazy. c = scale
+  // log2 e > 0.
+  XPU_DEVICE void settle(int r, float top, float c) {
+    const float ninf = -__builtin_inff();
     const bool grow = (top - m[r]) * c > kLazy;  // m = -inf: any finite score
     if (__builtin_amdgcn_ballot_w64(grow)) {
       const float now = grow ? top : m[r];
@@ -178,7 +201,11 @@ template <int DT, int D, int R> struct Rows {
         for (int i = 0; i < 16; ++i) o[r][dt][i] *= a;
       m[r] = now;
     }
-    const float shift = m[r] == ninf ? 0.0f : -m[r] * c;  // no score yet: every p is 0
+  }
+  // p of the tile packed as the MFMA takes it, word i of pk[t] for registers 2 i
+  // and 2 i + 1, and their sum.
+  template <int T> XPU_DEVICE void powers(int r, const f32x16 (&s)[T], float c, u32x8 (&pk)[T]) {
+    const float shift = m[r] == -__builtin_inff() ? 0.0f : -m[r] * c;  // no score yet: every p is 0
     float part = 0.0f;
 #pragma unroll
     for (int t = 0; t < T; ++t)
@@ -190,6 +217,10 @@ template <int DT, int D, int R> struct Rows {
         part = add_pair<DT>(pk[t][i / 2], part);
       }
     sum[r] += part;
+  }
+  template <int T> XPU_DEVICE void softmax(int r, const f32x16 (&s)[T], float c, u32x8 (&pk)[T]) {
+    settle(r, largest<T>(s), c);
+    powers<T>(r, s, c, pk);
   }
 
   // O^T += V^T P^T for the tile at LDS offset vb, the reads one step (16 keys)
@@ -220,6 +251,55 @@ template <int DT, int D, int R> struct Rows {
         }
       __builtin_amdgcn_sched_barrier(0);
     }
+  }
+
+  // One wavefront's MFMAs leave its vector ALU free, so a tile's powers are
+  // formed between the MFMAs of the next tile's scores, and that tile's
+  // largest scores between those of P V. The order is given to the compiler
+  // instruction by instruction: reads first, then an MFMA, a read and a share
+  // of the vector work at a time.
+  template <int DS, int VALU, int TRANS, int N, int AHEAD> XPU_DEVICE static void interleave() {
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);  // LDS reads
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // an MFMA
+      __builtin_amdgcn_sched_group_barrier(0x100, DS, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
+      if (TRANS) __builtin_amdgcn_sched_group_barrier(0x400, TRANS, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  XPU_DEVICE void scores_powers(uint32_t kb, f32x16 (&next)[2], const f32x16 (&s)[2], float c, u32x8 (&pk)[2]) {
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) next[t][i] = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < kKs; ++ks)
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        next[t] = dma::mfma<DT>(*reinterpret_cast<const lds_u32x4 *>(kb + ka[ks] + 32u * t * kRow), q[0][ks], next[t]);
+    powers<2>(0, s, c, pk);
+    interleave<1, D == 128 ? 5 : 10, 0, 2 * kKs, 4>();
+  }
+  XPU_DEVICE float values_largest(uint32_t vb, const u32x8 (&pk)[2], const f32x16 (&next)[2]) {
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (uint32_t ks = 0; ks < 4; ++ks)
+#pragma unroll
+      for (uint32_t dt = 0; dt < kDt; ++dt) {
+        const uint32_t at = va[dt] + vb + 16u * ks * kRow;
+        const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at)));
+        const u32x2 hi =
+            __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at + 8u * kRow)));
+        const u32x8 &p = pk[ks / 2];
+        const uint32_t b = 4u * (ks % 2);
+        o[0][dt] = dma::mfma<DT>(u32x4{lo.x, lo.y, hi.x, hi.y}, u32x4{p[b], p[b + 1], p[b + 2], p[b + 3]}, o[0][dt]);
+      }
+    const float top = largest<2>(next);
+    interleave<2, 2, 0, 4 * kDt, 8>();
+    return top;
   }
 
   // A tile with a non-finite value in a row that some query does not see: the

@@ -49,71 +49,66 @@ template <int D> XPU_DEVICE void append(const AppendArgs &a) {
   }
 }
 
-// The moves of `count` rows (at most N loads of 512 / D rows each) of one
-// (layer, kv head, K or V): all are loaded before the first is stored, so they
-// may overlap in any order. Branch-free up to the stores, so that the loads
-// are in flight together: rows that do not move read the pool's first element.
-template <int D, int N>
-XPU_DEVICE void move_rows(const KeepArgs &a, uint16_t *pool, const uint32_t *table, const uint32_t *kept,
-                          uint32_t context, uint32_t nodes, uint32_t count) {
-  constexpr uint32_t kRpi = 512u / D, kCpr = D / 8;
-  const uint32_t lane = lane_id();
-  auto element = [&](uint32_t node) {
-    return element_of(a.pool, table, a.batch.table_pitch, static_cast<uint64_t>(context) + node, D);
-  };
-  uint32_t node[N];
-#pragma unroll
-  for (uint32_t i = 0; i < N; ++i) {
-    const uint32_t j = i * kRpi + lane / kCpr;
-    node[i] = kept[j < count ? j : 0u];
-  }
-  u32x4 held[N];
-  uint64_t to[N];
-  bool odd = false;
-#pragma unroll
-  for (uint32_t i = 0; i < N; ++i) {
-    const uint32_t j = i * kRpi + lane / kCpr;
-    const bool moves = j < count && node[i] != j;
-    const uint64_t from = element(node[i] < nodes ? node[i] : 0u), at = element(j);
-    const bool fine = node[i] < nodes && from != kNowhere && at != kNowhere;
-    to[i] = moves && fine ? at : kNowhere;
-    odd |= moves && !fine;
-    held[i] = *reinterpret_cast<const u32x4 *>(pool + (moves && fine ? from : 0u));
-  }
-  if (__builtin_amdgcn_ballot_w64(odd)) report(a.pool);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-#pragma unroll
-  for (uint32_t i = 0; i < N; ++i)
-    if (to[i] != kNowhere) *reinterpret_cast<u32x4 *>(pool + to[i]) = held[i];
-}
-
-// One wavefront per (layer, kv head, K or V) of a sequence.
+// Four (layer, kv head, K or V) parts of a sequence per block. All kept rows
+// of a part are loaded before the first is stored, so they may move in any
+// order: up to 16 rows a part is a wavefront's, with more the wavefronts take
+// 16 rows each of one part after the other and meet in between. Branch-free up
+// to the stores, so that the loads are in flight together: rows that do not
+// move read the pool's first element. The pages of the up to 64 nodes lie in
+// lanes 0 .. 4.
 template <int D> XPU_DEVICE void keep(const KeepArgs &a) {
-  constexpr uint32_t kRpi = 512u / D;
-  const uint32_t lane = lane_id();
-  const uint32_t per = a.pool.layers * a.pool.kv_heads * 2u;
-  const uint64_t index = static_cast<uint64_t>(blockIdx.x) * 4u + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t seq = static_cast<uint32_t>(index / per), part = static_cast<uint32_t>(index % per);
-  if (seq >= a.batch.n_seqs) return;
+  constexpr uint32_t kRpi = 512u / D, kCpr = D / 8, kLoads = 16u / kRpi;
+  const uint32_t lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t parts = a.pool.layers * a.pool.kv_heads * 2u, groups = (parts + 3u) / 4u;
+  const uint32_t seq = blockIdx.x / groups, group = blockIdx.x % groups;
   const uint32_t lo = __builtin_amdgcn_readfirstlane(a.batch.starts[seq]);
   const uint32_t hi = __builtin_amdgcn_readfirstlane(a.batch.starts[seq + 1]);
   const uint32_t context = __builtin_amdgcn_readfirstlane(a.batch.context[seq]);
   const uint32_t count = __builtin_amdgcn_readfirstlane(a.counts[seq]);
-  const bool ok = lo <= hi && hi <= a.batch.rows && count <= hi - lo && count <= 64u;
-  if (!ok) {
+  if (!(lo <= hi && hi <= a.batch.rows && count <= hi - lo && count <= 64u)) {
     report(a.pool);
     return;
   }
-  if (part == 0 && lane == 0 && a.new_context) a.new_context[seq] = context + count;
+  if (group == 0 && threadIdx.x == 0 && a.new_context) a.new_context[seq] = context + count;
   if (count == 0) return;  // no row to read the first entry of
-  const uint32_t head = part / 2u % a.pool.kv_heads, layer = part / 2u / a.pool.kv_heads;
-  uint16_t *pool = (part % 2u ? a.pool.v : a.pool.k) + layer * a.pool.layer_stride +
-                   static_cast<uint64_t>(head) * a.pool.page_size * D + lane % (D / 8) * 8u;
-  const uint32_t *table = a.batch.tables + static_cast<uint64_t>(seq) * a.batch.table_pitch, *kept = a.kept + lo;
-  // accepted paths are short: few loads where few rows are kept
-  if (count <= 2u * kRpi) move_rows<D, 2>(a, pool, table, kept, context, hi - lo, count);
-  else if (count <= 16u) move_rows<D, 16 / kRpi>(a, pool, table, kept, context, hi - lo, count);
-  else move_rows<D, 64 / kRpi>(a, pool, table, kept, context, hi - lo, count);
+  const uint32_t first_page = context >> a.pool.page_shift, within = context & (a.pool.page_size - 1u);
+  const uint64_t page = static_cast<uint64_t>(first_page) + lane;
+  const uint32_t entry = a.batch.tables[static_cast<uint64_t>(seq) * a.batch.table_pitch +
+                                        (page < a.batch.table_pitch ? page : a.batch.table_pitch - 1u)];
+  const uint32_t id = page < a.batch.table_pitch ? entry : ~0u;
+  // the element of node `node` in a layer, kNowhere for a page that is not there
+  auto element = [&](uint32_t node) {
+    const uint32_t at = within + node;
+    const uint32_t p = __shfl(id, static_cast<int>(at >> a.pool.page_shift));
+    return p < a.pool.n_pages ? p * a.pool.page_stride + (at & (a.pool.page_size - 1u)) * D : kNowhere;
+  };
+  const bool apart = count <= 16u;  // the wavefronts work on parts of their own
+  bool odd = false;
+  for (uint32_t step = 0; step < (apart ? 1u : 4u); ++step) {
+    const uint32_t part = group * 4u + (apart ? wave : step), row = apart ? 0u : wave * 16u;
+    const uint32_t head = part / 2u % a.pool.kv_heads, layer = part / 2u / a.pool.kv_heads;
+    uint16_t *pool = (part % 2u ? a.pool.v : a.pool.k) + static_cast<uint64_t>(head) * a.pool.page_size * D +
+                     lane % kCpr * 8u + (layer < a.pool.layers ? layer * a.pool.layer_stride : 0u);
+    u32x4 held[kLoads];
+    uint64_t to[kLoads];
+#pragma unroll
+    for (uint32_t i = 0; i < kLoads; ++i) {
+      const uint32_t j = row + i * kRpi + lane / kCpr;
+      const uint32_t node = a.kept[lo + (j < count ? j : 0u)];
+      const bool moves = j < count && node != j, exists = node < hi - lo && node < 64u;
+      const uint64_t from = element(exists ? node : 0u), at = element(j);
+      const bool fine = exists && from != kNowhere && at != kNowhere;
+      to[i] = moves && fine && part < parts ? at : kNowhere;
+      odd |= moves && !fine;
+      held[i] = *reinterpret_cast<const u32x4 *>(pool + (to[i] != kNowhere ? from : 0u));
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (!apart) __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < kLoads; ++i)
+      if (to[i] != kNowhere) *reinterpret_cast<u32x4 *>(pool + to[i]) = held[i];
+  }
+  if (__builtin_amdgcn_ballot_w64(odd)) report(a.pool);
 }
 
 // Block (piece, pair, layer and K or V): 256 x 16 x 4 bytes of a page per step.

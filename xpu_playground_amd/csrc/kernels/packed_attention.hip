@@ -11,22 +11,68 @@
 #include "attention_core.hpp"
 #include "cache_types.hpp"
 
-#include <type_traits>
-
 namespace xpu {
 namespace att {
 
-// The sequence that owns slot `slot` of the work list, where sequence s has
-// the slots from starts[s] / tile + s on (tile = 1 << shift queries): at least
-// as many as it has tiles, and known without a sum over the sequences. -1: none.
-XPU_DEVICE int32_t sequence_of_slot(const uint32_t *starts, uint32_t n_seqs, uint32_t shift, uint32_t slot) {
+struct Work {
+  int32_t seq;       // -1: none
+  uint32_t first_q;  // of the sequence's queries
+  uint32_t q_lo, q_hi, k_lo, k_hi;
+};
+
+// Rows of sequence i, both kinds; starts that do not ascend or pass the rows
+// make it one without queries, and nothing of it is touched.
+XPU_DEVICE void rows_of(const PackedArgs &a, uint32_t i, Work &w) {
+  w.q_lo = a.q_starts[i];
+  w.q_hi = a.q_starts[i + 1];
+  w.k_lo = a.k_starts[i];
+  w.k_hi = a.k_starts[i + 1];
+  if (w.q_lo > w.q_hi || w.q_hi > a.q_rows || w.k_lo > w.k_hi || w.k_hi > a.k_rows) w.q_hi = w.q_lo;
+}
+
+// Work item `rank` of up to 64 sequences, a lane each: the query tiles (1 <<
+// shift queries) of all sequences by their place in the sequence, the last
+// places first, since a tile's keys are those before it. With f(j) tiles at
+// place j or behind it, the item's place is the last j with f(j) > rank, and
+// its sequence the (rank - f(j + 1))-th that has a tile there.
+XPU_DEVICE Work heaviest_first(const PackedArgs &a, uint32_t shift, uint32_t rank) {
+  Work w{};
+  if (lane_id() < a.n_seqs) rows_of(a, lane_id(), w);
+  const uint32_t tiles = (w.q_hi - w.q_lo + (1u << shift) - 1u) >> shift;
+  uint32_t place = 0, behind = 0;  // the place found so far; f(place + 1) once it is final
+  if (wave_total(tiles) <= rank) return {-1, 0, 0, 0, 0, 0};
+  for (uint32_t bit = 1u << (31u - __builtin_clz(a.q_rows >> shift | 1u)); bit; bit >>= 1) {
+    const uint32_t next = place + bit;
+    if (wave_total(tiles > next ? tiles - next : 0u) > rank) place = next;
+  }
+  behind = wave_total(tiles > place + 1u ? tiles - place - 1u : 0u);
+  const uint64_t have = __builtin_amdgcn_ballot_w64(tiles > place);
+  const uint32_t nth = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(have >> 32),
+                                                 __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(have), 0u));
+  const uint32_t l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(tiles > place && nth == rank - behind));
+  auto of = [&](uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(v, l)); };
+  return {static_cast<int32_t>(l), place << shift, of(w.q_lo), of(w.q_hi), of(w.k_lo), of(w.k_hi)};
+}
+
+// Work item `slot` of any number of sequences, the last first: sequence s has
+// the slots from (starts[s] >> shift) + s on, at least as many as it has tiles,
+// and known without a sum over the sequences.
+XPU_DEVICE Work by_slot(const PackedArgs &a, uint32_t shift, uint32_t slot) {
   int32_t s = -1;
-  for (uint32_t at = 0; at < n_seqs; at += 64) {
+  for (uint32_t at = 0; at < a.n_seqs; at += 64) {
     const uint32_t i = at + lane_id();
-    const bool before = i < n_seqs && (starts[i] >> shift) + i <= slot;
+    const bool before = i < a.n_seqs && (a.q_starts[i] >> shift) + i <= slot;
     s += __builtin_popcountll(__builtin_amdgcn_ballot_w64(before));
   }
-  return __builtin_amdgcn_readfirstlane(s);
+  Work w{};
+  w.seq = __builtin_amdgcn_readfirstlane(s);
+  if (s < 0) return w;
+  rows_of(a, static_cast<uint32_t>(w.seq), w);
+  for (uint32_t *v : {&w.q_lo, &w.q_hi, &w.k_lo, &w.k_hi}) *v = __builtin_amdgcn_readfirstlane(*v);
+  const uint32_t base = (w.q_lo >> shift) + static_cast<uint32_t>(w.seq);
+  if (base > slot || (slot - base) << shift >= w.q_hi - w.q_lo) w.seq = -1;
+  w.first_q = (slot - base) << shift;
+  return w;
 }
 
 template <int DT, int D> XPU_DEVICE void packed_attention(const PackedArgs &a) {
@@ -41,8 +87,7 @@ template <int DT, int D> XPU_DEVICE void packed_attention(const PackedArgs &a) {
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
   // Blocks are dealt to the 8 XCDs in turn: a kv head stays on one XCD (its K
-  // and V in that L2) where the head count allows; within it the last slots,
-  // the heaviest tiles of a sequence, come first.
+  // and V in that L2) where the head count allows.
   const uint32_t group = a.heads / a.kv_heads, packs = group >> a.pack_shift;
   uint32_t kvh, rest;
   if (a.kv_heads % 8u == 0) {
@@ -53,19 +98,13 @@ template <int DT, int D> XPU_DEVICE void packed_attention(const PackedArgs &a) {
     kvh = blockIdx.x % a.kv_heads;
     rest = blockIdx.x / a.kv_heads;
   }
-  const uint32_t slot = a.slots - 1u - rest / packs, qt_shift = 7u - a.pack_shift, q_tile = 1u << qt_shift;
-  const uint32_t head = kvh * group + (rest % packs << a.pack_shift) + (wave & (1u << a.pack_shift) - 1u);
-
-  const int32_t seq = sequence_of_slot(a.q_starts, a.n_seqs, qt_shift, slot);
-  if (seq < 0) return;
-  const uint32_t q_lo = __builtin_amdgcn_readfirstlane(a.q_starts[seq]);
-  const uint32_t q_hi = __builtin_amdgcn_readfirstlane(a.q_starts[seq + 1]);
-  const uint32_t k_lo = __builtin_amdgcn_readfirstlane(a.k_starts[seq]);
-  const uint32_t k_hi = __builtin_amdgcn_readfirstlane(a.k_starts[seq + 1]);
-  // starts that do not ascend or pass the rows: nothing of the sequence is touched
-  if (q_lo > q_hi || q_hi > a.q_rows || k_lo > k_hi || k_hi > a.k_rows || (q_lo >> qt_shift) + seq > slot) return;
-  const uint32_t first_q = (slot - ((q_lo >> qt_shift) + seq)) << qt_shift, n_q = q_hi - q_lo, n_k = k_hi - k_lo;
-  if (first_q >= n_q) return;
+  const uint32_t qt_shift = 7u - a.pack_shift, q_tile = 1u << qt_shift;
+  const uint32_t head = kvh * group + (rest % packs << a.pack_shift) + (wave & ((1u << a.pack_shift) - 1u));
+  const Work work = a.n_seqs <= 64u ? heaviest_first(a, qt_shift, rest / packs)
+                                    : by_slot(a, qt_shift, a.slots - 1u - rest / packs);
+  if (work.seq < 0) return;
+  const uint32_t first_q = work.first_q, q_lo = work.q_lo, k_lo = work.k_lo;
+  const uint32_t n_q = work.q_hi - q_lo, n_k = work.k_hi - k_lo;
   const int32_t shift = static_cast<int32_t>(n_k) - static_cast<int32_t>(n_q);
   const uint32_t t0 = first_q + 32u * (wave >> a.pack_shift);  // the wave's first query
   // keys of the block and of the wave: 0 .. seen - 1
@@ -79,7 +118,19 @@ template <int DT, int D> XPU_DEVICE void packed_attention(const PackedArgs &a) {
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(lds));
   Rows<DT, D, 1> rows;
   rows.init(lds0);
-  rows.load_q(0, a.q + (q_lo + min(t, n_q - 1u)) * a.q_stride + head * D);
+  // The queries come through the second stage, whole rows at a time, laid out
+  // as a tile's K rows: 32 rows per wave, rows past the sequence as zeros.
+  constexpr uint32_t kQDma = 32u / kRpi;
+  if (t0 < n_q) {
+    const i32x4 rq = rsrc(a.q + (q_lo + static_cast<uint64_t>(t0)) * a.q_stride + head * D,
+                          static_cast<int64_t>((min(n_q - t0, 32u) - 1u) * a.q_stride + D) * 2);
+#pragma unroll
+    for (uint32_t j = 0; j < kQDma; ++j) {
+      const uint32_t row = kRpi * j + lane / kCpr;
+      dma16(lds0 + kStage + (wave * kQDma + j) * 1024u, rq,
+            row * static_cast<uint32_t>(a.q_stride) * 2u + 16u * ((lane % kCpr) ^ k_swz<D>(row)));
+    }
+  }
 
   // DMA of the wave's share of a tile: instruction j fills LDS rows kRpi
   // (kDma wave + j) .., lane -> physical chunk lane % kCpr of row lane / kCpr.
@@ -93,52 +144,97 @@ template <int DT, int D> XPU_DEVICE void packed_attention(const PackedArgs &a) {
   }
   const uint16_t *k_head = a.k + static_cast<uint64_t>(k_lo) * a.k_stride + kvh * D;
   const uint16_t *v_head = a.v + static_cast<uint64_t>(k_lo) * a.v_stride + kvh * D;
-  auto issue = [&](uint32_t tile, uint32_t stage) {
+  auto issue = [&](uint32_t tile, bool k, bool v) {
+    if (tile >= n_tiles) return;
     const uint64_t first = static_cast<uint64_t>(tile) * kKeys;
     const uint32_t live = min(n_seen - tile * kKeys, kKeys);
-    const i32x4 rk = rsrc(k_head + first * a.k_stride, static_cast<int64_t>((live - 1u) * a.k_stride + D) * 2);
-    const i32x4 rv = rsrc(v_head + first * a.v_stride, static_cast<int64_t>((live - 1u) * a.v_stride + D) * 2);
-    const uint32_t at = lds0 + stage * kStage + wave * kDma * 1024u;
+    const uint32_t at = lds0 + (tile & 1u) * kStage + wave * kDma * 1024u;
+    if (k) {
+      const i32x4 r = rsrc(k_head + first * a.k_stride, static_cast<int64_t>((live - 1u) * a.k_stride + D) * 2);
 #pragma unroll
-    for (uint32_t j = 0; j < kDma; ++j) dma16(at + j * 1024u, rk, k_off[j]);
+      for (uint32_t j = 0; j < kDma; ++j) dma16(at + j * 1024u, r, k_off[j]);
+    }
+    if (v) {
+      const i32x4 r = rsrc(v_head + first * a.v_stride, static_cast<int64_t>((live - 1u) * a.v_stride + D) * 2);
 #pragma unroll
-    for (uint32_t j = 0; j < kDma; ++j) dma16(at + kTile + j * 1024u, rv, v_off[j]);
+      for (uint32_t j = 0; j < kDma; ++j) dma16(at + kTile + j * 1024u, r, v_off[j]);
+    }
   };
 
-  // one tile of keys; the stage is a constant, so the LDS reads' addresses are
-  // registers and constant offsets
-  auto step = [&](uint32_t tile, auto stage_of) {
-    constexpr uint32_t stage = stage_of, kb = stage * kStage, vb = kb + kTile;
-    // whether some query of the block does not see some key of the tile
-    const bool edge = static_cast<int32_t>(tile * kKeys + kKeys - 1u) > static_cast<int32_t>(first_q) + shift;
-    wait_vmcnt<0>();
-    if (edge) {  // the V rows that this wave staged, before the barrier that publishes them
-      bool bad = false;
-#pragma unroll
-      for (uint32_t j = 0; j < kDma; ++j) {
-        const u32x4 w = *reinterpret_cast<const lds_u32x4 *>(lds0 + vb + (wave * kDma + j) * 1024u + lane * 16u);
-        bad |= nonfinite<DT>(w.x) || nonfinite<DT>(w.y) || nonfinite<DT>(w.z) || nonfinite<DT>(w.w);
-      }
-      const bool any = __builtin_amdgcn_ballot_w64(bad) != 0;
-      if (lane == 0) flags[stage][wave] = any;
+  // Tiles that every query of the block sees in whole: the scores of a tile are
+  // formed during the softmax of the one before (scores_powers), so K runs one
+  // tile ahead of V. One barrier a tile, which publishes K of the next and V of
+  // this one and says that their predecessors' stages are read. The stage is
+  // a constant of the two alternating halves of the loop, so the LDS reads'
+  // addresses are registers and constant offsets.
+  const int32_t all = static_cast<int32_t>(first_q) + shift + 1;  // keys that every query sees
+  const uint32_t whole = min(all < 0 ? 0u : static_cast<uint32_t>(all) / kKeys, n_tiles);
+  uint32_t tile = 0;
+  issue(0, true, true);
+  if (n_tiles) wait_vmcnt<2 * kDma>();
+  else wait_vmcnt<0>();
+  rows.read_q(kStage + wave * kQDma * 1024u);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // before the barrier that frees the stage
+  if (whole) {
+    wait_vmcnt<kDma>();
+    __syncthreads();  // the queries are read, K of the first tile is there
+    if (whole > 1) issue(1, true, false);
+    f32x16 s0[2], s1[2];
+    rows.template scores<2, false>(0, 0, 0, s0);
+    float top = Rows<DT, D, 1>::template largest<2>(s0);
+    u32x8 pk[1][2];
+    auto turn = [&](auto stage_of, f32x16 (&s)[2], f32x16 (&next)[2]) {
+      constexpr uint32_t kb = (stage_of ^ 1u) * kStage, vb = stage_of * kStage + kTile;
+      wait_vmcnt<0>();
+      __syncthreads();
+      issue(tile + stage_of + 1, false, true);
+      issue(tile + stage_of + 2, true, false);
+      rows.settle(0, top, a.scale_log2e);
+      rows.scores_powers(kb, next, s, a.scale_log2e, pk[0]);
+      top = rows.values_largest(vb, pk[0], next);
+    };
+    for (; tile + 2 < whole; tile += 2) {
+      turn(std::integral_constant<uint32_t, 0>{}, s0, s1);
+      turn(std::integral_constant<uint32_t, 1>{}, s1, s0);
     }
+    // the scores of `tile` are there, and K of the next was asked for (but not behind a single one)
+    wait_vmcnt<0>();
     __syncthreads();
-    if (tile + 1 < n_tiles) issue(tile + 1, stage ^ 1u);
+    issue(tile + 1, whole == 1, true);
+    rows.settle(0, top, a.scale_log2e);
+    rows.template powers<2>(0, s0, a.scale_log2e, pk[0]);
+    rows.template values<2>(kTile, pk);
+    ++tile;
+  }
+
+  // The last tiles, among them those that some query does not see in whole.
+  for (; tile < n_tiles; ++tile) {
+    const uint32_t kb = (tile & 1u) * kStage, vb = kb + kTile;
+    wait_vmcnt<0>();
+    bool bad = false;  // the V rows that this wave staged, before the barrier that publishes them
+#pragma unroll
+    for (uint32_t j = 0; j < kDma; ++j) {
+      const u32x4 w = *reinterpret_cast<const lds_u32x4 *>(lds0 + vb + (wave * kDma + j) * 1024u + lane * 16u);
+      bad |= nonfinite<DT>(w.x) || nonfinite<DT>(w.y) || nonfinite<DT>(w.z) || nonfinite<DT>(w.w);
+    }
+    const bool any = __builtin_amdgcn_ballot_w64(bad) != 0;
+    if (lane == 0) flags[tile & 1u][wave] = any;
+    __syncthreads();
+    issue(tile + 1, true, true);
     const bool mine = tile < wave_tiles;
     u32x8 pk[1][2];
     uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
     if (mine) {
       f32x16 s[2];
       rows.template scores<2, false>(0, kb, 0, s);
-      if (static_cast<int32_t>(tile * kKeys + kKeys - 1u) > static_cast<int32_t>(t0) + shift) {  // wave-uniform
-        const int32_t last = static_cast<int32_t>(t) + shift - static_cast<int32_t>(tile * kKeys);
-        seen[0] = mask_to(last);
-        seen[1] = mask_to(last - 32);
-        Rows<DT, D, 1>::template mask<2>(s, seen);
-      }
+      const int32_t last = static_cast<int32_t>(t) + shift - static_cast<int32_t>(tile * kKeys);
+      seen[0] = mask_to(last);
+      seen[1] = mask_to(last - 32);
+      Rows<DT, D, 1>::template mask<2>(s, seen);
       rows.template softmax<2>(0, s, a.scale_log2e, pk[0]);
     }
-    if (edge && __builtin_expect(flags[stage][0] | flags[stage][1] | flags[stage][2] | flags[stage][3], 0)) {
+    const uint32_t *f = flags[tile & 1u];
+    if (__builtin_expect(__builtin_amdgcn_readfirstlane(f[0] | f[1] | f[2] | f[3]), 0)) {
       // the same in every wavefront: all read the rows before any clears its own
       if (mine) {
         rows.add_apart(lds0 + vb, 0, pk[0][0], seen[0]);
@@ -149,11 +245,6 @@ template <int DT, int D> XPU_DEVICE void packed_attention(const PackedArgs &a) {
       __syncthreads();
     }
     if (mine) rows.template values<2>(vb, pk);
-  };
-  if (n_tiles) issue(0, 0);
-  for (uint32_t tile = 0; tile < n_tiles; tile += 2) {
-    step(tile, std::integral_constant<uint32_t, 0>{});
-    if (tile + 1 < n_tiles) step(tile + 1, std::integral_constant<uint32_t, 1>{});
   }
   const float total = rows.total(0);
   if (t < n_q)  // a query that sees no key: 0

@@ -20,8 +20,6 @@
 #include "attention_core.hpp"
 #include "cache_types.hpp"
 
-#include <type_traits>
-
 namespace xpu {
 namespace att {
 
@@ -48,24 +46,6 @@ XPU_DEVICE Sequence uniform_sequence(const BatchArgs &b, uint32_t page_size, uin
   s.bad = __builtin_amdgcn_readfirstlane(s.bad);
   return s;
 }
-
-// Sums of lanes 0 .. own, with DPP moves: shifts within rows of 16 lanes, then
-// the rows' last lanes broadcast to the rows behind them.
-XPU_DEVICE uint32_t sum_upto(uint32_t v) {
-  auto add = [&](auto ctrl, auto rows) {
-    v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), ctrl.value, rows.value, 0xf, false));
-  };
-  using std::integral_constant;
-  constexpr integral_constant<int, 0xf> all;
-  add(integral_constant<int, 0x111>{}, all);  // row_shr:1, 2, 4, 8
-  add(integral_constant<int, 0x112>{}, all);
-  add(integral_constant<int, 0x114>{}, all);
-  add(integral_constant<int, 0x118>{}, all);
-  add(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});  // row_bcast:15 to rows 1 and 3
-  add(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});  // row_bcast:31 to rows 2 and 3
-  return v;
-}
-XPU_DEVICE uint32_t wave_total(uint32_t v) { return __builtin_amdgcn_readlane(sum_upto(v), 63); }
 
 // How the keys are cut: every chunk has at most `most` tiles, so that the
 // chunks of all sequences and row tiles are at most target + the row tiles.
