@@ -345,16 +345,28 @@ template <int DT, int D, int R> struct Rows {
   // The sum over both half-waves of each query.
   XPU_DEVICE float total(int r) const { return sum[r] + xor32_f(sum[r]); }
 
-  // Row of sub-tile r times `by`, rounded to the storage type.
-  XPU_DEVICE void store(int r, uint16_t *row, float by) const {
-    const uint32_t hh = lane_id() >> 5;
+  // The 32 rows of sub-tile 0, each query's times its `by` and rounded to the
+  // storage type, to `rows` rows of memory `stride` elements apart. Through 32
+  // kRow bytes of LDS at address `at` that belong to the wavefront, so that
+  // whole rows are stored (the lanes' own 8-byte pieces took twice the time of
+  // all else in a short prompt's block).
+  XPU_DEVICE void store(uint32_t at, float by, uint16_t *to, uint64_t stride, uint32_t rows) const {
+    constexpr uint32_t kCpr = D / 8, kRpi = 512u / D;
+    const uint32_t lane = lane_id(), row = lane & 31u;
 #pragma unroll
     for (uint32_t dt = 0; dt < kDt; ++dt)
 #pragma unroll
       for (uint32_t w = 0; w < 4; ++w)
-        *reinterpret_cast<u32x2 *>(row + 32u * dt + 8u * w + 4u * hh) =
-            u32x2{dma::cvt_pack<DT>(o[r][dt][4 * w] * by, o[r][dt][4 * w + 1] * by),
-                  dma::cvt_pack<DT>(o[r][dt][4 * w + 2] * by, o[r][dt][4 * w + 3] * by)};
+        *reinterpret_cast<lds_u32x2 *>(at + row * kRow + 16u * ((4u * dt + w) ^ k_swz<D>(row)) + 8u * (lane >> 5)) =
+            u32x2{dma::cvt_pack<DT>(o[0][dt][4 * w] * by, o[0][dt][4 * w + 1] * by),
+                  dma::cvt_pack<DT>(o[0][dt][4 * w + 2] * by, o[0][dt][4 * w + 3] * by)};
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (uint32_t j = 0; j < 32u / kRpi; ++j) {
+      const uint32_t r = j * kRpi + lane / kCpr;
+      const u32x4 v = *reinterpret_cast<const lds_u32x4 *>(at + r * kRow + 16u * ((lane % kCpr) ^ k_swz<D>(r)));
+      if (r < rows) *reinterpret_cast<u32x4 *>(to + r * stride + lane % kCpr * 8u) = v;
+    }
   }
 };
 

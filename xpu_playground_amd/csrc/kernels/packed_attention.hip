@@ -246,9 +246,12 @@ template <int DT, int D> XPU_DEVICE void packed_attention(const PackedArgs &a) {
     }
     if (mine) rows.template values<2>(vb, pk);
   }
+  // the stage that the last tile is not in: no wavefront reads it any more
+  if (t0 >= n_q) return;
   const float total = rows.total(0);
-  if (t < n_q)  // a query that sees no key: 0
-    rows.store(0, a.out + (q_lo + t) * a.out_stride + head * D, static_cast<int32_t>(t) + shift < 0 ? 0.0f : 1.0f / total);
+  rows.store(lds0 + (n_tiles & 1u) * kStage + wave * 32u * 2u * D,
+             static_cast<int32_t>(t) + shift < 0 ? 0.0f : 1.0f / total,  // a query that sees no key: 0
+             a.out + (q_lo + static_cast<uint64_t>(t0)) * a.out_stride + head * D, a.out_stride, min(n_q - t0, 32u));
 }
 
 }  // namespace att
