@@ -22,7 +22,8 @@
  * on the operands has to be ordered against the runtime's stream by the
  * caller. Operands are device pointers of the runtime's device, 16-byte
  * aligned where they hold rows, 4-byte (visible: 8-byte) aligned where they
- * hold numbers. Row strides are in elements, multiples of 8. Host-side
+ * hold numbers; what a call writes must not overlap what it reads, unless the
+ * call says so. Row strides are in elements, multiples of 8. Host-side
  * arguments that are wrong fail with XPU_ERR_INVALID before any launch. The
  * numbers that live on the device (starts, context, tables, kept, counts)
  * are checked by the kernels: nothing outside the described buffers is read
@@ -56,8 +57,10 @@ typedef struct {
 /* Sequences with new rows. Sequence s has rows starts[s] .. starts[s + 1] - 1
  * of the row operands (none, one or many), at positions context[s], context[s]
  * + 1, ... of its cache; its position p lies in page tables[s * table_pitch +
- * p / page_size], slot p % page_size. starts ascend from any first row;
- * rows that belong to no sequence are left as they are. A table entry that no
+ * p / page_size], slot p % page_size. starts (n_seqs + 1) ascend from any first
+ * row; rows that belong to no sequence are left as they are. A sequence whose
+ * starts descend or pass `rows` has no rows; rows that several sequences then
+ * claim get any one's result, or none and status. A table entry that no
  * position needs may hold anything. */
 typedef struct {
   uint32_t n_seqs;
@@ -104,7 +107,8 @@ int xpu_tree_attention_workspace(const xpu_runtime *rt, const xpu_cache *cache, 
  * starts[s] + j] held before the call, for j < counts[s] (at most 64 and at
  * most the sequence's rows). kept names nodes 0 .. 63 of the sequence's rows,
  * in any order and more than once if need be. The
- * positions behind the kept ones hold what they held. new_context (NULL, or
+ * positions behind the kept ones hold what they held. kept has `rows` entries;
+ * those past a sequence's count are not looked at. new_context (NULL, or
  * n_seqs entries apart from context): context[s] + counts[s]. A sequence with
  * a count that does not fit is left alone, and so is a row with a node or a
  * page that does not exist; both set status. The pages of the batch's rows

@@ -105,7 +105,8 @@ def attend(q, k, v, seen, scale, dtype, merges=4):
 
 
 def check(got, want, tol, what=""):
-    bad = ~((np.abs(got - want) <= tol) | (np.isnan(got) & np.isnan(want)) | (got == want))
+    with np.errstate(invalid="ignore"):  # infinities
+        bad = ~((np.abs(got - want) <= tol) | (np.isnan(got) & np.isnan(want)) | (got == want))
     if bad.any():
         i = tuple(int(x[0]) for x in np.nonzero(bad))
         raise AssertionError(f"{what}: {int(bad.sum())} of {bad.size} values outside the bound, first at {i}: "

@@ -198,6 +198,22 @@ def test_unseen_nodes_take_no_part(rt, dtype, d, bad, context):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("context", [40, 700, 2999, 9000])
+@pytest.mark.parametrize("heads,kv", [(4, 2), (40, 2)])
+def test_infinities_that_rows_see(rt, dtype, context, heads, kv):
+    """An infinite value comes out as itself, wherever the cut puts it; the other dims are not touched."""
+    case = Case([3, 4], [context, 50], heads, kv, 64, 16, dtype, 18, masked=False)
+    want, tol = case.expected(64 ** -0.5)
+    spots = sorted({0, context // 2, context - 1, context})
+    for dim, at in enumerate(spots):
+        case.v[1, case.tables[0, at // 16], :, at % 16, 7 + dim] = INF[dtype] | (0x8000 if dim % 2 else 0)
+        want[:3, :, 7 + dim] = -np.inf if dim % 2 else np.inf
+    got, status = case.run(rt)
+    check(values(got, dtype), want, tol)
+    assert status == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("what", ["id", "id in the middle", "context", "nodes"])
 def test_pages_and_lengths_that_do_not_exist(rt, dtype, what):
     """That sequence's rows are NaN and the status says so; the others are served."""
@@ -231,6 +247,38 @@ def test_lengths_beyond_all_bounds(rt):
     got, _ = case.run(rt)
     check(values(got, xpu.BF16)[:3], want[:3], tol[:3])
     assert (got[3:] == GUARD).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("nodes, contexts, heads, kv, d", [
+    ([1], [17000], 3, 1, 128),            # a row of 128 chunks or more: sixteen wavefronts, an odd head
+    ([2, 1, 2], [900, 17000, 130], 4, 4, 64),  # the same, with rows of few chunks and of none
+    ([41], [1500], 32, 8, 64),            # four wavefronts a join
+    ([110], [700], 32, 4, 64),            # one
+    ([1, 70, 41], [3000, 0, 700], 30, 10, 128),
+])
+def test_joins_by_any_number_of_wavefronts(rt, dtype, nodes, contexts, heads, kv, d):
+    Case(nodes, contexts, heads, kv, d, 64, dtype, 21, masked=False, layers=2, spare=1).verify(rt)
+
+
+def test_more_work_than_the_workspace_holds(rt):
+    """Starts that go back give more work items than ascending ones could:
+    rows that would be joined from behind the workspace are left, with status."""
+    heads, d, page, n = 8, 64, 16, 4001
+    rows, pitch = 20, 61
+    starts = u32([0, 16] * ((n - 1) // 2) + [16, 20])  # the first rows 2000 times, then the last ones
+    with Buffers(rt) as b:
+        status, pool = b.up(u32([0])), np.zeros((1, 1, page, d), np.uint16)
+        cache = xpu.Cache(xpu.BF16, 1, 1, d, page, 1, b.up(pool), b.up(pool), status)
+        batch = xpu.Batch(n, rows, pitch, b.up(np.zeros((n, pitch), np.uint32)), b.up(starts), b.up(u32([0] * (n - 1) + [960])))
+        out = np.full((rows, heads, d), GUARD, np.uint16)
+        size, to = rt.tree_attention_workspace(cache, batch, heads), b.up(out)
+        rt.tree_attention(cache=cache, batch=batch, layer=0, heads=heads, q=b.up(np.zeros_like(out)), out=to,
+                          workspace=b.alloc(size), workspace_bytes=size)
+        rt.synchronize()
+        got = rt.download(to, out.size, np.uint16).reshape(out.shape)
+        assert int(rt.download(status, 1, np.uint32)[0]) == 1
+    assert (got[16:] == GUARD).all() and (got[:16] == 0).all()
 
 
 @pytest.mark.parametrize("dtype", TYPES)

@@ -104,13 +104,13 @@ xpu::BatchArgs batch_of(const xpu_batch &b) { return {b.tables, b.starts, b.cont
 
 template <typename A>
 int launch(xpu_runtime *rt, const std::string &kernel, uint64_t grid, const A &args, uint32_t grid_y = 1,
-           const uint32_t *more = nullptr) {
+           const uint32_t *more = nullptr, uint32_t block = 256) {
   if (grid > kMostBlocks) return set_error(XPU_ERR_INVALID, kernel + ": too many rows for one launch");
   const xpu::KernelInfo *k = rt->find_exact(kernel);
   if (!k) return set_error(XPU_ERR_NOT_FOUND, "kernel is absent from module: " + kernel);
   XPU_HIP_RETURN(hipSetDevice(rt->device));
   const xpu_kernel_arg list[] = {{sizeof(A), &args}, {4, more}};
-  return rt->launch(*k, static_cast<uint32_t>(grid), grid_y, 256, 0, list, more ? 2 : 1);
+  return rt->launch(*k, static_cast<uint32_t>(grid), grid_y, block, 0, list, more ? 2 : 1);
 }
 
 const char *type_name(int32_t dtype) { return dtype == XPU_DTYPE_FP16 ? "fp16" : "bf16"; }
@@ -122,7 +122,9 @@ struct TreePlan {
   uint32_t target = 1;     // chunks aimed at per kv head
   uint32_t least = 4;      // tiles of 32 keys in a chunk, one for each wavefront
   uint64_t slots = 0;      // work items per kv head, at most
-  uint64_t bytes = 0;
+  uint64_t bytes = 0;      // of the workspace; 0: the keys are not cut
+  uint64_t joins = 0;      // pairs of heads of all rows, each joined by
+  uint32_t join_waves = 1; // so many wavefronts
 };
 
 TreePlan tree_plan(const xpu_runtime &rt, const xpu_cache &c, const xpu_batch &b, uint32_t heads) {
@@ -143,13 +145,20 @@ TreePlan tree_plan(const xpu_runtime &rt, const xpu_cache &c, const xpu_batch &b
   const bool cut = tiles > p.least;
   p.slots = row_tiles + (cut ? p.target : 0);
   p.bytes = cut ? p.slots * c.kv_heads * (32ull * p.sub_tiles * (c.head_dim + 2)) * 4 : 0;
+  // the fewer joins, the more wavefronts for each, which read its chunks side
+  // by side: one above 6 per unit (48 sequences of 4 nodes 76.3 us, with four
+  // 77.9; of 2 nodes, 6 per unit, both 73.1; of 1 node 71.2 and 70.1), four
+  // above 2 per unit (48 of 1 node 70.1, with eight 71.3; one of 16 nodes at
+  // 8000 positions, half per unit, 22.0 and 20.3), eight below, sixteen where
+  // a row can have 128 chunks (32000 positions of 2 kv heads: 33.7 us with
+  // four, 24.5 with eight, 20.6 with sixteen; of 8 kv heads, 64 chunks: 28.7,
+  // 27.8, 28.6)
+  p.joins = b.rows * ((heads + 1ull) / 2);
+  p.join_waves = p.joins > 6ull * rt.compute_units ? 1
+                 : p.joins > 2ull * rt.compute_units ? 4
+                 : std::min<uint64_t>(p.target, tiles / p.least) < 128 ? 8 : 16;
   return p;
 }
-
-// Wavefronts that join a row's chunks: four for a few rows, whose chunks are
-// many (12 rows and heads of 256 chunks: 34.3 -> 28.5 us in all), one for
-// others (1536 of a few chunks: 75.8 us with four, 74.5 with one).
-constexpr uint64_t kWideJoins = 128;
 
 }  // namespace
 
@@ -225,14 +234,15 @@ int xpu_tree_attention(xpu_runtime *rt, const xpu_cache *cache, const xpu_batch 
     a.heads = heads;
     a.target = plan.target;
     a.least = plan.least;
+    a.slots = static_cast<uint32_t>(plan.slots);
     a.scale_log2e = static_cast<float>(scale * kLog2e);
     const std::string form = std::string("_") + type_name(cache->dtype) + "_d" + std::to_string(cache->head_dim) +
                              "_r" + std::to_string(plan.sub_tiles);
     if (int rc = launch(rt, "xpu_tree_attention" + form, plan.slots * cache->kv_heads, a)) return rc;
     if (!plan.bytes) return XPU_OK;
-    const uint64_t joins = static_cast<uint64_t>(batch->rows) * heads;
-    return joins <= kWideJoins ? launch(rt, "xpu_tree_join" + form + "_w4", joins, a)
-                               : launch(rt, "xpu_tree_join" + form, (joins + 3) / 4, a);
+    const std::string join = "xpu_tree_join" + form + "_w" + std::to_string(plan.join_waves);
+    return plan.join_waves > 1 ? launch(rt, join, plan.joins, a, 1, nullptr, 64 * plan.join_waves)
+                               : launch(rt, join, (plan.joins + 3) / 4, a);
   });
 }
 

@@ -37,16 +37,6 @@ template <int R> XPU_DEVICE Sequence sequence(const BatchArgs &b, uint32_t page_
   return s;
 }
 
-// Sequence i, the same in every lane, in scalar registers.
-template <int R>
-XPU_DEVICE Sequence uniform_sequence(const BatchArgs &b, uint32_t page_size, uint32_t group, uint32_t i) {
-  Sequence s = sequence<R>(b, page_size, group, i);
-  for (uint32_t *v : {&s.first, &s.n, &s.context, &s.end, &s.row_tiles, &s.tiles})
-    *v = __builtin_amdgcn_readfirstlane(*v);
-  s.bad = __builtin_amdgcn_readfirstlane(s.bad);
-  return s;
-}
-
 // How the keys are cut: every chunk has at most `most` tiles, so that the
 // chunks of all sequences and row tiles are at most target + the row tiles.
 // The work items are numbered sequence by sequence, chunk by chunk, and row
@@ -58,6 +48,7 @@ XPU_DEVICE Sequence uniform_sequence(const BatchArgs &b, uint32_t page_size, uin
 struct Place {
   int32_t seq;  // -1: none
   uint32_t first, chunks;
+  Sequence s;
 };
 template <int R, typename Is> XPU_DEVICE Place find(const TreeArgs &a, uint32_t group, Is &&is) {
   const uint32_t n = a.batch.n_seqs;
@@ -86,14 +77,22 @@ template <int R, typename Is> XPU_DEVICE Place find(const TreeArgs &a, uint32_t 
     const uint64_t hit = __builtin_amdgcn_ballot_w64(at + lane_id() < n && is(first, count, s));
     if (hit) {
       const uint32_t l = __builtin_ctzll(hit);
-      return {static_cast<int32_t>(at + l), static_cast<uint32_t>(__builtin_amdgcn_readlane(first, l)),
-              static_cast<uint32_t>(__builtin_amdgcn_readlane(chunks, l))};
+      auto of = [&](uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(v, l)); };
+      Place p{static_cast<int32_t>(at + l), of(first), of(chunks), {}};
+      p.s.first = of(s.first);
+      p.s.n = of(s.n);
+      p.s.context = of(s.context);
+      p.s.end = of(s.end);
+      p.s.bad = of(s.bad);
+      p.s.row_tiles = of(s.row_tiles);
+      p.s.tiles = of(s.tiles);
+      return p;
     }
     if ((at += 64) >= n) break;
     before += __builtin_amdgcn_readlane(upto, 63);
     s = of_lane(at);
   }
-  return {-1, 0, 0};
+  return {-1, 0, 0, {}};
 }
 
 // Floats of one work item's partial result: 32 R rows of D sums, then their
@@ -120,7 +119,7 @@ template <int DT, int D, int R> XPU_DEVICE void tree_attention(const TreeArgs &a
   });
   if (place.seq < 0) return;
   const uint32_t seq = static_cast<uint32_t>(place.seq);
-  const Sequence s = uniform_sequence<R>(a.batch, a.pool.page_size, group, seq);
+  const Sequence &s = place.s;
   const uint32_t row_tile = (item - place.first) % s.row_tiles, chunk = (item - place.first) / s.row_tiles;
   const uint32_t rows_in = min(s.n * group - row_tile * 32u * R, 32u * R);
   // the chunk's tiles, and the wave's share of them
@@ -341,84 +340,100 @@ template <int DT, int D, int R> XPU_DEVICE void tree_attention(const TreeArgs &a
   }
 }
 
-// Adds the chunks of the rows whose keys were cut: W wavefronts per (row,
-// query head), each a W-th of the chunks. A lane takes one chunk's (max, sum)
-// of 64, then the half-waves every other chunk's outputs, D / 32 dims per
-// lane, kAhead loads in flight; the first of them go out with the (max, sum)
-// pairs, so that up to 2 kAhead chunks take one round trip to memory.
+// Reductions over each half-wave: partners l ^ 16, 8, 4, 2, 1 of wave_reduce.
+template <typename Op> XPU_DEVICE float half_reduce(float s, Op op) {
+  s = op(s, xor16_f(s));
+  s = op(s, xor8_f(s));
+  s = op(s, dpp_f<0x124>(s));  // row_ror:4
+  s = op(s, dpp_f<0x4E>(s));   // quad_perm [2,3,0,1]
+  return op(s, dpp_f<0xB1>(s));  // quad_perm [1,0,3,2]
+}
+
+// Adds the chunks of the rows whose keys were cut: W wavefronts, each a W-th
+// of the chunks, per row and two query heads, a half-wave each (half as many
+// wavefronts, so that a batch's rows are one round of them on the chip). A lane
+// takes one chunk's (max, sum) of 32, then D / 32 dims of every chunk's output,
+// kAhead loads in flight, the first of which go out with the (max, sum) pairs.
 template <int DT, int D, int R, int W> XPU_DEVICE void tree_join(const TreeArgs &a) {
   constexpr uint32_t kPer = D / 32, kAhead = 8;
   typedef float out_t __attribute__((ext_vector_type(kPer)));
-  const uint32_t lane = lane_id(), half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t index = W == 4 ? blockIdx.x : blockIdx.x * 4u + wave;
-  const uint32_t row_at = index / a.heads, head = index % a.heads, group = a.heads / a.pool.kv_heads;
+  const uint32_t lane = lane_id(), half = lane >> 5, in_half = lane & 31u;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pairs = (a.heads + 1u) / 2u;
+  const uint32_t index = W > 1 ? blockIdx.x : blockIdx.x * 4u + wave;
+  const uint32_t row_at = index / pairs, head = min(index % pairs * 2u + half, a.heads - 1u);
+  const bool spare = index % pairs * 2u + half >= a.heads;  // an odd number of heads
+  const uint32_t group = a.heads / a.pool.kv_heads;
   if (row_at >= a.batch.rows) return;
   const Place place = find<R>(a, group, [&](uint32_t, uint32_t, const Sequence &s) {
     return row_at >= s.first && row_at - s.first < s.n;
   });
   if (place.seq < 0 || place.chunks < 2) return;
-  const Sequence s = uniform_sequence<R>(a.batch, a.pool.page_size, group, static_cast<uint32_t>(place.seq));
-  const uint32_t kvh = head / group, row = (row_at - s.first) * group + head % group;
-  const uint32_t in = row % (32u * R);
-  const uint32_t begin = W == 4 ? place.chunks * wave / 4u : 0u, chunks = W == 4 ? place.chunks * (wave + 1u) / 4u : place.chunks;
+  const Sequence &s = place.s;
+  // with starts that do not ascend there can be more work items than the workspace has
+  if (place.first + static_cast<uint64_t>(s.row_tiles) * place.chunks > a.slots) {
+    if (lane == 0 && a.pool.status) *a.pool.status = 1u;
+    return;
+  }
+  const uint32_t kvh = head / group, row = (row_at - s.first) * group + head % group, in = row % (32u * R);
+  const uint32_t begin = W > 1 ? place.chunks * wave / W : 0u;
+  const uint32_t end = W > 1 ? place.chunks * (wave + 1u) / W : place.chunks;
   const uint64_t step = static_cast<uint64_t>(s.row_tiles) * a.pool.kv_heads * kPartial<D, R>;
   const float *part = a.partial + (static_cast<uint64_t>(place.first + row / (32u * R)) * a.pool.kv_heads + kvh) * kPartial<D, R>;
-  const float *ms = part + 32u * R * D + 2u * in, *os = part + in * D + (lane & 31u) * kPer;
+  const float *ms = part + 32u * R * D + 2u * in, *os = part + in * D + in_half * kPer;
   const float ninf = -__builtin_inff();
   float top = ninf, sum = 0.0f;
   out_t o = {}, v[kAhead];
-  auto ask = [&](uint32_t c) {  // past the last chunk: it again, with weight 0
+  auto ask = [&](uint32_t c) {  // past the last chunk: it again, not counted
 #pragma unroll
-    for (uint32_t i = 0; i < kAhead; ++i)
-      v[i] = *reinterpret_cast<const out_t *>(os + min(c + 2u * i + half, chunks - 1u) * step);
+    for (uint32_t i = 0; i < kAhead; ++i) v[i] = *reinterpret_cast<const out_t *>(os + min(c + i, end - 1u) * step);
   };
-  for (uint32_t c0 = begin; c0 < chunks; c0 += 64) {
-    const uint32_t mine = c0 + lane;
-    const dma::f32x2 ml = *reinterpret_cast<const dma::f32x2 *>(ms + min(mine, chunks - 1u) * step);
+  for (uint32_t c0 = begin; c0 < end; c0 += 32) {
+    const uint32_t mine = c0 + in_half, n = min(end - c0, 32u);
+    const dma::f32x2 ml = *reinterpret_cast<const dma::f32x2 *>(ms + min(mine, end - 1u) * step);
     ask(c0);
-    const float m = mine < chunks ? ml.x : ninf, l = mine < chunks ? ml.y : 0.0f;
-    const float now = fmaxf(top, wave_reduce(m, [](float x, float y) { return fmaxf(x, y); }));
+    const float m = mine < end ? ml.x : ninf, l = mine < end ? ml.y : 0.0f;
+    const float now = fmaxf(top, half_reduce(m, [](float x, float y) { return fmaxf(x, y); }));
     const float old = top == ninf ? 0.0f : __builtin_amdgcn_exp2f((top - now) * a.scale_log2e);
     const float x = m == ninf ? 0.0f : __builtin_amdgcn_exp2f((m - now) * a.scale_log2e);
     // without a finite score the sum is zeros or NaN, which stay
-    sum = (top == ninf ? sum : sum * old) + wave_butterfly(m == ninf ? l : l * x);
+    sum = (top == ninf ? sum : sum * old) +
+          half_reduce(m == ninf ? l : l * x, [](float x, float y) { return x + y; });
     o *= old;
     top = now;
-    const uint32_t n = min(chunks - c0, 64u);
-    for (uint32_t j = 0; j < n; j += 2u * kAhead) {
+    for (uint32_t j = 0; j < n; j += kAhead) {
       if (j) ask(c0 + j);
 #pragma unroll
       for (uint32_t i = 0; i < kAhead; ++i) {
-        const float even = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), j + 2u * i));
-        const float odd = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), j + 2u * i + 1u));
-        const float w = half ? odd : even;
-#pragma unroll
-        for (uint32_t d = 0; d < kPer; ++d) o[d] = __builtin_fmaf(v[i][d], w, o[d]);
+        if (j + i >= n) break;
+        const float lo = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), j + i));
+        const float hi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 32u + j + i));
+        o += v[i] * (half ? hi : lo);
       }
     }
   }
-  if constexpr (W == 4) {
-    __shared__ float tops[4], sums[4];
-    __shared__ __align__(16) out_t outs[4][64];
-    if (lane == 0) tops[wave] = top, sums[wave] = sum;
+  if constexpr (W > 1) {
+    __shared__ float tops[W][64], sums[W][64];
+    __shared__ __align__(16) out_t outs[W][64];
+    tops[wave][lane] = top;
+    sums[wave][lane] = sum;
     outs[wave][lane] = o;
     __syncthreads();
     if (wave) return;
-    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    top = tops[0][lane];
+#pragma unroll
+    for (uint32_t w = 1; w < W; ++w) top = fmaxf(top, tops[w][lane]);
     sum = 0.0f;
     o = 0.0f;
 #pragma unroll
-    for (uint32_t w = 0; w < 4; ++w) {
-      const float x = tops[w] == ninf ? 0.0f : __builtin_amdgcn_exp2f((tops[w] - top) * a.scale_log2e);
-      sum += tops[w] == ninf ? sums[w] : sums[w] * x;
+    for (uint32_t w = 0; w < W; ++w) {
+      const float t = tops[w][lane], x = t == ninf ? 0.0f : __builtin_amdgcn_exp2f((t - top) * a.scale_log2e);
+      sum += t == ninf ? sums[w][lane] : sums[w][lane] * x;
       o += outs[w][lane] * x;
     }
   }
-  const float by = 1.0f / sum;  // a row that sees nothing has at most 64 positions, which are never cut
-#pragma unroll
-  for (uint32_t d = 0; d < kPer; ++d) o[d] = (o[d] + xor32_f(o[d])) * by;
-  if (half) return;
-  uint16_t *to = a.out + row_at * a.out_stride + head * D + lane * kPer;
+  if (spare) return;
+  o *= 1.0f / sum;  // a row that sees nothing has at most 64 positions, which are never cut
+  uint16_t *to = a.out + row_at * a.out_stride + head * D + in_half * kPer;
   if constexpr (kPer == 4)
     *reinterpret_cast<u32x2 *>(to) = u32x2{dma::cvt_pack<DT>(o[0], o[1]), dma::cvt_pack<DT>(o[2], o[3])};
   else
@@ -428,16 +443,18 @@ template <int DT, int D, int R, int W> XPU_DEVICE void tree_join(const TreeArgs 
 }  // namespace att
 }  // namespace xpu
 
+#define XPU_TREE_JOIN(T, NAME, D, R, W, BLOCK)                                                            \
+  extern "C" __global__ __launch_bounds__(BLOCK) void xpu_tree_join_##NAME##_w##W(xpu::TreeArgs a) {      \
+    xpu::att::tree_join<xpu::T, D, R, W>(a);                                                              \
+  }
 #define XPU_TREE_ATTENTION(T, NAME, D, R)                                                                 \
   extern "C" __global__ __launch_bounds__(256, 2) void xpu_tree_attention_##NAME(xpu::TreeArgs a) {       \
     xpu::att::tree_attention<xpu::T, D, R>(a);                                                            \
   }                                                                                                       \
-  extern "C" __global__ __launch_bounds__(256) void xpu_tree_join_##NAME(xpu::TreeArgs a) {               \
-    xpu::att::tree_join<xpu::T, D, R, 1>(a);                                                              \
-  }                                                                                                       \
-  extern "C" __global__ __launch_bounds__(256) void xpu_tree_join_##NAME##_w4(xpu::TreeArgs a) {          \
-    xpu::att::tree_join<xpu::T, D, R, 4>(a);                                                              \
-  }
+  XPU_TREE_JOIN(T, NAME, D, R, 1, 256)                                                                    \
+  XPU_TREE_JOIN(T, NAME, D, R, 4, 256)                                                                    \
+  XPU_TREE_JOIN(T, NAME, D, R, 8, 512)                                                                    \
+  XPU_TREE_JOIN(T, NAME, D, R, 16, 1024)
 XPU_TREE_ATTENTION(kBf16, bf16_d128_r1, 128, 1)
 XPU_TREE_ATTENTION(kFp16, fp16_d128_r1, 128, 1)
 XPU_TREE_ATTENTION(kBf16, bf16_d64_r1, 64, 1)
