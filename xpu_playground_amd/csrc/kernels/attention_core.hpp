@@ -349,7 +349,8 @@ template <int DT, int D, int R> struct Rows {
   // storage type, to `rows` rows of memory `stride` elements apart. Through 32
   // kRow bytes of LDS at address `at` that belong to the wavefront, so that
   // whole rows are stored (the lanes' own 8-byte pieces took twice the time of
-  // all else in a short prompt's block).
+  // all else in a short prompt's block), past the L2, which keeps the keys (24
+  // sequences of 17 .. 1500 rows, 32 heads: 96.4 us with, 93.3 past it).
   XPU_DEVICE void store(uint32_t at, float by, uint16_t *to, uint64_t stride, uint32_t rows) const {
     constexpr uint32_t kCpr = D / 8, kRpi = 512u / D;
     const uint32_t lane = lane_id(), row = lane & 31u;
@@ -365,7 +366,7 @@ template <int DT, int D, int R> struct Rows {
     for (uint32_t j = 0; j < 32u / kRpi; ++j) {
       const uint32_t r = j * kRpi + lane / kCpr;
       const u32x4 v = *reinterpret_cast<const lds_u32x4 *>(at + r * kRow + 16u * ((lane % kCpr) ^ k_swz<D>(r)));
-      if (r < rows) *reinterpret_cast<u32x4 *>(to + r * stride + lane % kCpr * 8u) = v;
+      if (r < rows) __builtin_nontemporal_store(v, reinterpret_cast<u32x4 *>(to + r * stride + lane % kCpr * 8u));
     }
   }
 };

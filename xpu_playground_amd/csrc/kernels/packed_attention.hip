@@ -221,30 +221,35 @@ template <int DT, int D> XPU_DEVICE void packed_attention(const PackedArgs &a) {
     if (lane == 0) flags[tile & 1u][wave] = any;
     __syncthreads();
     issue(tile + 1, true, true);
-    const bool mine = tile < wave_tiles;
-    u32x8 pk[1][2];
-    uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
-    if (mine) {
-      f32x16 s[2];
-      rows.template scores<2, false>(0, kb, 0, s);
-      const int32_t last = static_cast<int32_t>(t) + shift - static_cast<int32_t>(tile * kKeys);
-      seen[0] = mask_to(last);
-      seen[1] = mask_to(last - 32);
-      Rows<DT, D, 1>::template mask<2>(s, seen);
-      rows.template softmax<2>(0, s, a.scale_log2e, pk[0]);
-    }
+    // a wave whose queries see the first half only forms no scores of the other
+    // (32 sequences of 17 .. 200 rows, 32 heads: 16.9 us without this, 15.8)
+    const bool mine = tile < wave_tiles, half = wave_seen <= static_cast<int32_t>(tile * kKeys) + 32;
+    const int32_t last = static_cast<int32_t>(t) + shift - static_cast<int32_t>(tile * kKeys);
+    u32x8 pk[1][2], pk_half[1][1];
+    auto scored = [&](auto parts, auto &to) {
+      f32x16 s[parts];
+      uint32_t seen[parts];
+#pragma unroll
+      for (int32_t i = 0; i < parts; ++i) seen[i] = mask_to(last - 32 * i);
+      rows.template scores<parts, false>(0, kb, 0, s);
+      Rows<DT, D, 1>::template mask<parts>(s, seen);
+      rows.template softmax<parts>(0, s, a.scale_log2e, to[0]);
+    };
+    if (mine && half) scored(std::integral_constant<int32_t, 1>{}, pk_half);
+    if (mine && !half) scored(std::integral_constant<int32_t, 2>{}, pk);
     const uint32_t *f = flags[tile & 1u];
     if (__builtin_expect(__builtin_amdgcn_readfirstlane(f[0] | f[1] | f[2] | f[3]), 0)) {
       // the same in every wavefront: all read the rows before any clears its own
       if (mine) {
-        rows.add_apart(lds0 + vb, 0, pk[0][0], seen[0]);
-        rows.add_apart(lds0 + vb + kTile / 2u, 0, pk[0][1], seen[1]);
+        rows.add_apart(lds0 + vb, 0, half ? pk_half[0][0] : pk[0][0], mask_to(last));
+        if (!half) rows.add_apart(lds0 + vb + kTile / 2u, 0, pk[0][1], mask_to(last - 32));
       }
       __syncthreads();
       Rows<DT, D, 1>::clear_apart(lds0 + vb + wave * kTile / 4u, kKeys / 4u);
       __syncthreads();
     }
-    if (mine) rows.template values<2>(vb, pk);
+    if (mine && half) rows.template values<1>(vb, pk_half);
+    if (mine && !half) rows.template values<2>(vb, pk);
   }
   // the stage that the last tile is not in: no wavefront reads it any more
   if (t0 >= n_q) return;
