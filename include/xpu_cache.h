@@ -110,7 +110,7 @@ int xpu_tree_attention_workspace(const xpu_runtime *rt, const xpu_cache *cache, 
  * positions behind the kept ones hold what they held. kept has `rows` entries;
  * those past a sequence's count are not looked at. new_context (NULL, or
  * n_seqs entries apart from context): context[s] + counts[s]. A sequence with
- * a count that does not fit is left alone, and so is a row with a node or a
+ * a count that does not fit is left alone, its new_context too, and so is a row with a node or a
  * page that does not exist; both set status. The pages of the batch's rows
  * must be the sequence's own. */
 int xpu_cache_keep(xpu_runtime *rt, const xpu_cache *cache, const xpu_batch *batch, const uint32_t *kept,

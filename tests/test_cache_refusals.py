@@ -105,7 +105,7 @@ def test_append_refuses(kwargs, word):
 
 @pytest.mark.parametrize("kwargs,word", [
     (dict(layer=2), "layer"), (dict(heads=3), "heads"), (dict(heads=0), "heads"), (dict(scale=0.0), "scale"),
-    (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
+    (dict(scale=-1.0), "scale"), (dict(scale=3e38), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
     (dict(q=None), "null q"), (dict(out=None), "null out"), (dict(q=A + 4), "aligned"), (dict(q_stride=255), "q_stride"),
     (dict(out_stride=248), "out_stride"), (dict(visible=A + 4), "visible"), (dict(out=6 * A), "overlap"),
     (dict(out=6 * A + 256), "overlap"), (dict(b=batch(rows=1 << 25), out=1 << 50), "rows")])
@@ -116,7 +116,8 @@ def test_tree_attention_refuses(kwargs, word):
 
 @pytest.mark.parametrize("kwargs,word", [
     (dict(kept=None), "null"), (dict(counts=None), "null"), (dict(kept=A + 2), "aligned"), (dict(new=A + 2), "aligned"),
-    (dict(new=5 * A), "overlap"), (dict(new=7 * A + 4), "overlap"), (dict(new=4 * A + 8), "overlap")])
+    (dict(new=5 * A), "overlap"), (dict(new=7 * A + 4), "overlap"), (dict(new=4 * A + 8), "overlap"),
+    (dict(new=6 * A + 36), "overlap"), (dict(b=batch(rows=0, starts=None)), "null"), (dict(b=batch(rows=0), counts=None), "null")])
 def test_keep_refuses(kwargs, word):
     rc, text = keep(**kwargs)
     assert rc == INVALID and word in text and "runtime" not in text, text
@@ -147,6 +148,13 @@ def test_prompt_attention_refuses(over, word):
 def test_prompt_attention_refuses_pointers(kwargs, word):
     rc, text = prompt(**kwargs)
     assert rc == INVALID and word in text and "runtime" not in text, text
+
+
+def test_page_ids_that_32_bits_do_not_hold():
+    for ids in ([-1], np.array([-1]), np.array([1 << 32]), [0.5], [[1]]):
+        with pytest.raises(ValueError, match="page ids"):
+            xpu.page_ids(ids)
+    assert xpu.page_ids([]).dtype == np.uint32 and list(xpu.page_ids(np.array([3, 0xFFFFFFFF]))) == [3, 0xFFFFFFFF]
 
 
 def test_null_descriptions():

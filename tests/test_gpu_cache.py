@@ -142,6 +142,74 @@ def test_keep_leaves_what_does_not_fit(rt):
         pool.verify(status=1)
 
 
+def test_keep_without_rows_gives_the_contexts(rt):
+    with Buffers(rt) as b:
+        pool, n = Pool(rt, b, 2), 70
+        batch = xpu.Batch(n, 0, 1, b.up(u32([0] * n)), b.up(u32([0] * (n + 1))), b.up(u32(range(n))))
+        new = b.up(u32([GUARD] * n))
+        rt.cache_keep(pool.cache, batch, None, b.up(u32([0] * n)), new)
+        pool.verify()
+        assert list(rt.download(new, n, np.uint32)) == list(range(n))
+
+
+@pytest.mark.parametrize("dtype", [xpu.BF16, xpu.FP16])
+def test_decode_steps_as_two_graphs(rt, dtype):
+    """Append, attention and the step to the next context captured together:
+    two graphs that hand the contexts to and fro, replayed with eager work
+    between, over a padded batch."""
+    kv, heads, d, page, n, pad = 2, 8, 128, 16, 3, 2
+    contexts, steps = [14, 300, 0], 6
+    rng = random.Random(8)
+    with Buffers(rt) as b:
+        sizes = [c + steps for c in contexts]
+        pool = Pool(rt, b, sum(-(-s // page) for s in sizes) + 1, kv, d, page, 1, dtype)
+        tables = tables_of(sizes, page, pool.n_pages, rng)
+        dt, starts = b.up(tables), b.up(u32([0, 1, 2, 3]))
+        both = [b.up(u32(contexts)), b.up(u32([GUARD] * n))]
+        rows = [np.full((n + pad, h, d), GUARD, np.uint16) for h in (heads, kv, kv)]
+        dq, dk, dv = (b.up(r) for r in rows)
+        out, kept, counts = b.up(rows[0]), b.up(u32([0] * (n + pad))), b.up(u32([1] * n))
+        batches = [xpu.Batch(n, n + pad, tables.shape[1], dt, starts, c) for c in both]
+        size = rt.tree_attention_workspace(pool.cache, batches[0], heads)
+        workspace, graphs = b.alloc(size), []
+        for i in range(2):
+            xpu.check(rt.lib.xpu_rt_capture_begin(rt.handle))
+            rt.cache_append(pool.cache, batches[i], 0, dk, dv)
+            rt.tree_attention(pool.cache, batches[i], 0, heads, dq, out, workspace, size)
+            rt.cache_keep(pool.cache, batches[i], kept, counts, both[1 - i])
+            graph = ctypes.c_void_p()
+            xpu.check(rt.lib.xpu_rt_capture_end(rt.handle, ctypes.byref(graph)))
+            graphs.append(graph)
+        for step in range(steps):
+            q, k, v = (normal(r[:n].shape, 30 + 3 * step + i, dtype) for i, r in enumerate(rows))
+            for ptr, part, whole in ((dq, q, rows[0]), (dk, k, rows[1]), (dv, v, rows[2])):
+                rt.copy_to(ptr, np.concatenate([part, whole[n:]]))
+            xpu.check(rt.lib.xpu_rt_graph_launch(rt.handle, graphs[step % 2]))
+            for s in range(n):
+                p, slot = pool.place(tables[s], contexts[s] + step)
+                pool.k[0, p, :, slot], pool.v[0, p, :, slot] = k[s], v[s]
+            pool.verify()
+            assert list(rt.download(both[(step + 1) % 2], n, np.uint32)) == [c + step + 1 for c in contexts]
+            got = rt.download(out, (n + pad) * heads * d, np.uint16).reshape(n + pad, heads, d)
+            assert (got[n:] == GUARD).all()
+            for s in range(n):
+                at = [pool.place(tables[s], p) for p in range(contexts[s] + step + 1)]
+                for h in range(heads):
+                    keys, vals = (np.array([x[0, p, h // 4, slot] for p, slot in at]) for x in (pool.k, pool.v))
+                    want, tol = attend(values(q[s:s + 1, h], dtype), values(keys, dtype), values(vals, dtype),
+                                       np.ones((1, len(at)), bool), d ** -0.5, dtype, 64)
+                    check(values(got[s:s + 1, h], dtype), want, tol, f"step {step} sequence {s} head {h}")
+            # the same again, eagerly, into another context
+            spare = b.alloc(4 * n)
+            rt.tree_attention(pool.cache, batches[step % 2], 0, heads, dq, out, workspace, size)
+            rt.cache_keep(pool.cache, batches[step % 2], kept, counts, spare)
+            rt.synchronize()
+            again = rt.download(out, got.size, np.uint16).reshape(got.shape)
+            assert np.array_equal(again, got)
+        for graph in graphs:
+            rt.lib.xpu_rt_graph_destroy(graph)
+
+
 @pytest.mark.parametrize("d,kv,page,n", [(64, 1, 16, 1), (64, 3, 16, 7), (128, 8, 64, 20), (128, 2, 256, 3), (64, 1, 16, 900)])
 def test_copy(rt, d, kv, page, n):
     """Up to more pairs than one launch takes."""

@@ -381,3 +381,13 @@ def test_many_sequences(rt):
     rng = random.Random(16)
     nodes = [rng.choice([0, 1, 1, 2, 5]) for _ in range(150)]
     Case(nodes, [rng.randint(0, 60) for _ in nodes], 2, 1, 64, 16, xpu.FP16, 16).verify(rt)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads, d, few", [(2, 64, 1), (8, 128, 9)])
+def test_many_sequences_with_long_ones_among_them(rt, dtype, heads, d, few):
+    """The long ones' keys are cut, whichever 64 sequences they are among."""
+    nodes, contexts = [few] * 140, [5] * 140
+    for s, n, c in ((3, 20, 3000), (64, 1, 9000), (127, 11, 700), (139, 30, 5000)):
+        nodes[s], contexts[s] = n, c
+    Case(nodes, contexts, heads, 1, d, 32, dtype, 18, layers=2).verify(rt)

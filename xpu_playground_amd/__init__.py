@@ -52,6 +52,18 @@ class Qwen3Config(ctypes.Structure):
     ]
 
 
+def page_ids(ids):
+    """Page ids as the C calls take them: one-dimensional uint32."""
+    import numpy as np
+
+    a = np.asarray(ids)
+    if a.ndim != 1 or (a.size and a.dtype.kind not in "iu"):
+        raise ValueError("page ids must be a list of integers")
+    if a.size and not 0 <= int(a.min()) <= int(a.max()) <= 0xFFFFFFFF:
+        raise ValueError("page ids must be unsigned 32-bit integers")
+    return np.ascontiguousarray(a, dtype=np.uint32)
+
+
 class Cache(ctypes.Structure):
     """xpu_cache (include/xpu_cache.h): the pages of a KV cache. k and v are
     device addresses; without strides the pools are [layers][n_pages]
@@ -487,11 +499,9 @@ class Runtime:
 
     def cache_copy(self, cache: Cache, src, dst) -> None:
         """src, dst: page ids on the host (arrays or lists of one length)."""
-        import numpy as np
-
-        s, d = (np.ascontiguousarray(ids, dtype=np.uint32) for ids in (src, dst))
-        if s.ndim != 1 or s.shape != d.shape:
-            raise ValueError("src and dst must be one-dimensional and of one length")
+        s, d = page_ids(src), page_ids(dst)
+        if len(s) != len(d):
+            raise ValueError("src and dst must be of one length")
         check(self.lib.xpu_cache_copy(self.handle, cache, s.ctypes.data, d.ctypes.data, len(s)))
 
     def prompt_attention(self, packed: Packed, q: int, k: int, v: int, out: int) -> None:

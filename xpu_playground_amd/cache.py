@@ -11,14 +11,7 @@ from ctypes import c_uint32, c_void_p
 
 import numpy as np
 
-from . import check, library
-
-
-def _ids(ids) -> np.ndarray:
-    a = np.ascontiguousarray(ids, dtype=np.uint32)
-    if a.ndim != 1:
-        raise ValueError("page ids must be one-dimensional")
-    return a
+from . import check, library, page_ids
 
 
 class Pages:
@@ -55,18 +48,18 @@ class Pages:
 
     def share(self, ids) -> None:
         """One holder more for each: a forked sequence holds the same pages."""
-        a = _ids(ids)
+        a = page_ids(ids)
         check(self.lib.xpu_pages_share(self.handle, a.ctypes.data, len(a)))
 
     def release(self, ids) -> None:
         """One holder less for each; pages without holders are free."""
-        a = _ids(ids)
+        a = page_ids(ids)
         check(self.lib.xpu_pages_release(self.handle, a.ctypes.data, len(a)))
 
     def own(self, ids) -> tuple[np.ndarray, np.ndarray, np.ndarray]:
         """(ids, src, dst): the pages as the caller's alone, and the copies
         src[i] -> dst[i] that Runtime.cache_copy has to make first."""
-        a = _ids(ids).copy()
+        a = page_ids(ids).copy()
         src, dst, n = np.empty(len(a), np.uint32), np.empty(len(a), np.uint32), c_uint32()
         check(self.lib.xpu_pages_own(self.handle, a.ctypes.data, len(a), src.ctypes.data, dst.ctypes.data,
                                      ctypes.byref(n)))
@@ -81,7 +74,7 @@ class Pages:
 
 def renumber(src, dst, ids) -> np.ndarray:
     """A table's ids after the moves of Pages.compact."""
-    s, d, a = _ids(src), _ids(dst), _ids(ids).copy()
+    s, d, a = page_ids(src), page_ids(dst), page_ids(ids).copy()
     if len(s) != len(d):
         raise ValueError("src and dst must be of one length")
     check(library().xpu_pages_renumber(s.ctypes.data, d.ctypes.data, len(s), a.ctypes.data, len(a)))

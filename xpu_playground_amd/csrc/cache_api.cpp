@@ -56,10 +56,11 @@ int check_cache(const char *name, const xpu_cache *c, bool memory) {
   return XPU_OK;
 }
 
-int check_batch(const char *name, const xpu_batch *b, bool memory) {
+// `idle`: a batch without rows has nothing to be done, so its memory may be anything.
+int check_batch(const char *name, const xpu_batch *b, bool memory, bool idle = true) {
   if (!b) return invalid(name, "null batch");
   if (b->rows >> 31 || b->n_seqs >> 24) return invalid(name, "at most 2^31 - 1 rows and 2^24 - 1 sequences");
-  if (!b->rows || !b->n_seqs) return XPU_OK;
+  if (!b->n_seqs || (idle && !b->rows)) return XPU_OK;
   if (!b->table_pitch) return invalid(name, "table_pitch must be positive");
   if (!memory) return XPU_OK;
   if (!b->tables || !b->starts || !b->context) return invalid(name, "null batch memory");
@@ -81,7 +82,8 @@ int check_rows(const char *name, const char *what, const void *p, uint64_t strid
 int check_heads(const char *name, uint32_t heads, uint32_t kv_heads, float scale) {
   if (!heads || !kv_heads || heads % kv_heads || heads > 65536)
     return invalid(name, "heads must be a positive multiple of kv_heads, at most 65536");
-  if (!(scale > 0) || !std::isfinite(scale)) return invalid(name, "scale must be positive and finite");
+  if (!(scale > 0) || !std::isfinite(static_cast<float>(scale * kLog2e)))
+    return invalid(name, "scale must be positive and finite, also times log2(e)");
   return XPU_OK;
 }
 
@@ -251,15 +253,16 @@ int xpu_cache_keep(xpu_runtime *rt, const xpu_cache *cache, const xpu_batch *bat
   static constexpr char name[] = "xpu_cache_keep";
   return guarded(name, [&] {
     if (int rc = check_cache(name, cache, true)) return rc;
-    if (int rc = check_batch(name, batch, true)) return rc;
-    if (!batch->rows || !batch->n_seqs) return check_runtime(name, rt);
-    if (!kept || !counts) return invalid(name, "null argument");
+    if (int rc = check_batch(name, batch, true, false)) return rc;
+    if (!batch->n_seqs) return check_runtime(name, rt);
+    if ((!kept && batch->rows) || !counts) return invalid(name, "null argument");
     if (!aligned(kept, 4) || !aligned(counts, 4) || !aligned(new_context, 4))
       return invalid(name, "kept, counts and new_context must be 4-byte aligned");
     const uint64_t list = 4ull * batch->n_seqs;
     if (new_context && (overlap(new_context, list, batch->context, list) || overlap(new_context, list, counts, list) ||
-                        overlap(new_context, list, batch->starts, list + 4)))
-      return invalid(name, "new_context must not overlap context, counts or starts");
+                        overlap(new_context, list, batch->starts, list + 4) ||
+                        (kept && overlap(new_context, list, kept, 4ull * batch->rows))))
+      return invalid(name, "new_context must not overlap context, counts, starts or kept");
     if (int rc = check_runtime(name, rt)) return rc;
     const xpu::KeepArgs a{pool_of(*cache), batch_of(*batch), kept, counts, new_context};
     const uint64_t groups = (static_cast<uint64_t>(cache->layers) * cache->kv_heads * 2 + 3) / 4;
