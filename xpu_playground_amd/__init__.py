@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import os
 import weakref
+from array import array
 from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_size_t, c_uint32, c_uint64, c_void_p
 
 PACKAGE_DIR = os.path.dirname(os.path.abspath(__file__))
@@ -56,12 +57,18 @@ def page_ids(ids):
     """Page ids as the C calls take them: one-dimensional uint32."""
     import numpy as np
 
-    a = np.asarray(ids)
-    if a.ndim != 1 or (a.size and a.dtype.kind not in "iu"):
-        raise ValueError("page ids must be a list of integers")
-    if a.size and not 0 <= int(a.min()) <= int(a.max()) <= 0xFFFFFFFF:
-        raise ValueError("page ids must be unsigned 32-bit integers")
-    return np.ascontiguousarray(a, dtype=np.uint32)
+    if not isinstance(ids, np.ndarray):
+        try:
+            ids = array("I", ids)
+            ids = np.frombuffer(ids, np.uint32) if ids else np.empty(0, np.uint32)
+        except (TypeError, OverflowError) as e:
+            raise ValueError(f"page ids must be a list of unsigned 32-bit integers: {e}") from None
+    elif ids.dtype != np.uint32:
+        if ids.size and (ids.dtype.kind not in "iu" or int(ids.min()) < 0 or int(ids.max()) > 0xFFFFFFFF):
+            raise ValueError("page ids must be unsigned 32-bit integers")
+    if ids.ndim != 1:
+        raise ValueError("page ids must be one-dimensional")
+    return np.ascontiguousarray(ids, dtype=np.uint32)
 
 
 class Cache(ctypes.Structure):
