@@ -7,7 +7,18 @@
 // (the group's largest such divisor) x 4 / P sub-tiles of the same sequence,
 // so that a sequence is cut into tiles of 128 / P queries: little is lost at
 // the ends of short sequences and at the diagonal. Key tiles of 64 are staged
-// by LDS-DMA, two stages of K then V, shared by the wavefronts.
+// by LDS-DMA, two stages of K then V, shared by the wavefronts; two blocks to
+// a compute unit (217 registers), so one's start and end fall into the other's
+// tiles. Work is dealt heaviest first, since a last heavy tile would run alone.
+//
+// Measured: 8192 rows, 32 heads on 8, D 128, 499 us or 1.10 PFLOP/s of the
+// causal half, 91% of what a large matrix product reaches here (the shader
+// clock, power-managed, is at 1.8 GHz with the MFMA busy in 65% of the cycles).
+// 24 sequences of 17 .. 1500 rows, the same heads, 93 us or 0.69 PFLOP/s: a
+// block has 8 tiles on average, and its queries' and result's way to memory
+// (14 us of the 93 without them) and its last, masked tile are not hidden.
+// 128 rows of 16 heads 7 us: one launch and a chain of loads. At D 64 the
+// powers bound it, 32 per lane for 16 MFMAs.
 #include "attention_core.hpp"
 #include "cache_types.hpp"
 
