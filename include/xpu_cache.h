@@ -60,7 +60,7 @@ typedef struct {
  * p / page_size], slot p % page_size. starts (n_seqs + 1) ascend from any first
  * row; rows that belong to no sequence are left as they are. A sequence whose
  * starts descend or pass `rows` has no rows; rows that several sequences then
- * claim get any one's result, or none and status. A table entry that no
+ * claim get any one's result or none. A table entry that no
  * position needs may hold anything. */
 typedef struct {
   uint32_t n_seqs;

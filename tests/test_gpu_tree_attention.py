@@ -261,6 +261,15 @@ def test_joins_by_any_number_of_wavefronts(rt, dtype, nodes, contexts, heads, kv
     Case(nodes, contexts, heads, kv, d, 64, dtype, 21, masked=False, layers=2, spare=1).verify(rt)
 
 
+@pytest.mark.parametrize("n, few, kv", [(1, 64, 8), (5, 64, 8), (20, 30, 8), (46, 3, 8), (60, 3, 8), (64, 30, 2), (64, 1, 16)])
+def test_ragged_batches_are_cut_to_fit_or_not(rt, n, few, kv):
+    """Every work item runs, and every row is written, however the rows fill a round of the chip."""
+    rng = random.Random(n * 100 + few)
+    nodes = [rng.randint(1, few) for _ in range(n)]
+    contexts = [int(60 * 80 ** rng.random()) for _ in range(n)]
+    Case(nodes, contexts, 2 * kv, kv, 64, 64, xpu.BF16, 23, layers=2).verify(rt)
+
+
 def test_more_work_than_the_workspace_holds(rt):
     """Starts that go back give more work items than ascending ones could:
     rows that would be joined from behind the workspace are left, with status."""

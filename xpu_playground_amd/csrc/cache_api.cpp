@@ -121,6 +121,7 @@ const char *type_name(int32_t dtype) { return dtype == XPU_DTYPE_FP16 ? "fp16" :
 // goes by what the host knows: numbers of rows and sequences, not lengths.
 struct TreePlan {
   uint32_t sub_tiles = 1;  // of 32 rows per block
+  uint32_t fit = 0;        // work items per kv head at most; 0: as `target` gives
   uint32_t target = 1;     // chunks aimed at per kv head
   uint32_t least = 4;      // tiles of 32 keys in a chunk, one for each wavefront
   uint64_t slots = 0;      // work items per kv head, at most
@@ -137,15 +138,21 @@ TreePlan tree_plan(const xpu_runtime &rt, const xpu_cache &c, const xpu_batch &b
   // 1 .. 26 nodes x 4 heads, 28 rows on average, 98.4 us in 32s and 90.5 in
   // 64s; 23 rows 93.8 and 90.5; 20 rows 86.8 and 88.2; 4 rows 69.5 and 72.7)
   p.sub_tiles = rows > 22ull * b.n_seqs ? 2 : 1;
-  // a compute unit holds two blocks; ragged sequences balance better on three
-  // per unit, dealt as they end (48 drafts 96.3 -> 90.4 us, four long ones
-  // 472 -> 415), a single one is cut evenly (32000 positions 28.2 us at two,
-  // 31.7 at three)
-  p.target = std::max(1u, (b.n_seqs > 1 ? 3 : 2) * rt.compute_units / c.kv_heads);
-  const uint64_t row_tiles = rows / (32 * p.sub_tiles) + b.n_seqs;
+  const uint64_t row_tiles = rows / (32 * p.sub_tiles) + b.n_seqs;  // at most
   const uint64_t tiles = (static_cast<uint64_t>(b.table_pitch) * c.page_size + 31) / 32;
   const bool cut = tiles > p.least;
-  p.slots = row_tiles + (cut ? p.target : 0);
+  // A compute unit holds two blocks. Cut into just as many as the chip holds,
+  // all run at once and end together, and none starts with nothing to do (four
+  // long drafts 375 us, with 3 blocks per unit dealt as others end 420; 16
+  // ragged ones of 1 .. 26 nodes 36.4 and 47.0; one token behind 32000
+  // positions 28.1 and 31.5, behind 16000 19.2 and 23.6). Where more than four
+  // fifths of them are row tiles, the chunks get too uneven: three per unit (48
+  // single tokens 70.0 us, and 79.8 cut to fit; 32 drafts of up to 8 nodes 53.4
+  // to fit and 56.0).
+  const uint64_t fit = 2 * rt.compute_units / c.kv_heads;
+  if (cut && b.n_seqs <= 64 && row_tiles <= fit * 4 / 5) p.fit = static_cast<uint32_t>(fit);
+  p.target = std::max(1u, 3 * rt.compute_units / c.kv_heads);
+  p.slots = p.fit ? fit : row_tiles + (cut ? p.target : 0);
   p.bytes = cut ? p.slots * c.kv_heads * (32ull * p.sub_tiles * (c.head_dim + 2)) * 4 : 0;
   // the fewer joins, the more wavefronts for each, which read its chunks side
   // by side: one above 6 per unit (48 sequences of 4 nodes 76.3 us, with four
@@ -158,7 +165,7 @@ TreePlan tree_plan(const xpu_runtime &rt, const xpu_cache &c, const xpu_batch &b
   p.joins = b.rows * ((heads + 1ull) / 2);
   p.join_waves = p.joins > 6ull * rt.compute_units ? 1
                  : p.joins > 2ull * rt.compute_units ? 4
-                 : std::min<uint64_t>(p.target, tiles / p.least) < 128 ? 8 : 16;
+                 : std::min<uint64_t>(p.fit ? p.fit : p.target, tiles / p.least) < 128 ? 8 : 16;
   return p;
 }
 
@@ -234,6 +241,7 @@ int xpu_tree_attention(xpu_runtime *rt, const xpu_cache *cache, const xpu_batch 
     a.q_stride = q_stride;
     a.out_stride = out_stride;
     a.heads = heads;
+    a.fit = plan.fit;
     a.target = plan.target;
     a.least = plan.least;
     a.slots = static_cast<uint32_t>(plan.slots);

@@ -75,7 +75,7 @@ struct TreeArgs {
   const uint64_t *visible;
   float *partial;
   uint64_t q_stride, out_stride;
-  uint32_t heads, target, least, slots;
+  uint32_t heads, fit, target, least, slots;
   float scale_log2e;
 };
 

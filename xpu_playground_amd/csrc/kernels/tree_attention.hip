@@ -23,9 +23,10 @@
 // up to 8000 positions 70 us, 5.65 TB/s; 48 drafts of 1 .. 26 nodes x 4 heads
 // the same way 89 us, 5.0 TB/s (the counters say that no key is read twice);
 // four drafts of 40 .. 64 nodes x 2 heads behind 90000 .. 131000 positions
-// 421 us, 4.45 TB/s, each key read by two blocks of 64 rows and 17% of them
-// twice from memory; one token behind 2100 positions 11.2 us, two launches
-// and their chains of loads, behind 32000 27.9 us, 4.7 TB/s. 128 rows to a
+// 378 us, 5.0 TB/s, each key read by two blocks of 64 rows and 17% of them
+// twice from memory; of 16 nodes there, one block a key, 295 us, 6.25 TB/s;
+// one token behind 2100 positions 11.5 us, two launches and their chains of
+// loads, behind 32000 28.1 us, 4.6 TB/s. 128 rows to a
 // block need more registers than there are (spills, 2272 us for the four
 // drafts); eight wavefronts over common tiles with barriers took 432 us, a
 // join in the last block to end instead of a second launch 18.4 us for the
@@ -50,8 +51,11 @@ template <int R> XPU_DEVICE Sequence sequence(const BatchArgs &b, uint32_t page_
   return s;
 }
 
-// How the keys are cut: every chunk has at most `most` tiles, so that the
-// chunks of all sequences and row tiles are at most target + the row tiles.
+// How the keys are cut: every chunk has at most `most` tiles. With `fit`, it is
+// (in six halvings, so nearly) the least with which the chunks of all sequences
+// (64 at most) and row tiles are at most fit: work / fit where that will do,
+// else between it and work / (fit - row tiles), which always does. Without,
+// work / target, which gives at most target + the row tiles.
 // The work items are numbered sequence by sequence, chunk by chunk, and row
 // tile by row tile within it, so that the row tiles that read the same keys
 // run side by side (and, with 8 kv heads, on one XCD). find() gives the
@@ -80,12 +84,27 @@ template <int R, typename Is> XPU_DEVICE Place find(const TreeArgs &a, uint32_t 
     if ((at += 64) >= n) break;
     s = of_lane(at);
   }
-  const uint64_t share = (work + a.target - 1) / a.target;
-  const uint32_t most = share < a.least ? a.least : static_cast<uint32_t>(share);
+  auto share = [&](uint32_t parts) {
+    const uint64_t w = (work + parts - 1u) / parts;
+    return w < a.least ? a.least : static_cast<uint32_t>(w < 0x7fffffffu ? w : 0x7fffffffu);
+  };
+  uint32_t most = share(a.fit ? a.fit : a.target);
+  auto fits = [&](uint32_t m) { return wave_total(s.row_tiles * ((s.tiles + m - 1u) / m)) <= a.fit; };
+  // (one row tile always fits; 0.3 us of a short call)
+  if (a.fit && (n > 1u || a.batch.rows * group > 32u * R) && !fits(most)) {
+    const uint32_t row_tiles = wave_total(s.row_tiles);
+    uint32_t too_few = most;
+    most = share(row_tiles < a.fit ? a.fit - row_tiles : 1u);
+    for (uint32_t i = 0; i < 6 && too_few + 1u < most; ++i) {
+      const uint32_t mid = too_few + (most - too_few) / 2u;
+      if (fits(mid)) most = mid;
+      else too_few = mid;
+    }
+  }
   uint32_t before = 0;
   if (n > 64) s = of_lane(0);
   for (uint32_t at = 0;;) {
-    const uint32_t chunks = (s.tiles + most - 1) / most, count = s.row_tiles * chunks;
+    const uint32_t chunks = (s.tiles + most - 1u) / most, count = s.row_tiles * chunks;
     const uint32_t upto = sum_upto(count), first = before + upto - count;
     const uint64_t hit = __builtin_amdgcn_ballot_w64(at + lane_id() < n && is(first, count, s));
     if (hit) {
