@@ -17,7 +17,7 @@
  * carries out the copies that forks and compaction ask for.
  *
  * Conventions: as xpu_kernels.h. Every launch is asynchronous on the
- * runtime's stream, allocates nothing and reads no device memory on the host,
+ * runtime's stream, allocates no device memory and reads none on the host,
  * so all of it can be captured (xpu_rt_capture_begin). Work of other streams
  * on the operands has to be ordered against the runtime's stream by the
  * caller. Operands are device pointers of the runtime's device, 16-byte
