@@ -1,0 +1,46 @@
+"""xpu_tree_attention where two rare things meet: rows that see nothing in
+sequences whose pages do not exist."""
+import numpy as np
+import pytest
+
+import xpu_playground_amd as xpu
+from cache_util import GUARD, Buffers, attend, check, normal, u32, values
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [xpu.BF16, xpu.FP16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("nodes,missing", [(3, 0), (20, 1), (40, 0), (40, 2), (64, 3)])
+def test_rows_that_see_nothing_of_missing_pages(rt, dtype, d, nodes, missing):
+    """No context, one row masked to nothing and one page past the pool: every
+    element of the sequence's rows is NaN, also those that wavefronts store
+    which did not meet the page. The sequence beside it is served, its row that
+    sees nothing with zeros."""
+    heads, kv, page, n_pages = 4, 2, 16, 9
+    pool_k, pool_v = (normal((1, n_pages, kv, page, d), s, dtype) for s in (1, 2))
+    tables = u32([[0, 1, 2, 3], [4, 5, 6, 7]])
+    tables[0, missing] = n_pages
+    rows = nodes + 5
+    masks = [(1 << i + 1) - 1 for i in range(nodes)] + [(1 << i + 1) - 1 for i in range(5)]
+    masks[1] = masks[nodes + 2] = 0
+    q = normal((rows, heads, d), 3, dtype)
+    print(f"tree attention d {d} dtype {dtype} nodes {nodes} missing page {missing}", flush=True)
+    with Buffers(rt) as b:
+        status = b.up(u32([0]))
+        cache = xpu.Cache(dtype, 1, kv, d, page, n_pages, b.up(pool_k), b.up(pool_v), status)
+        batch = xpu.Batch(2, rows, 4, b.up(tables), b.up(u32([0, nodes, rows])), b.up(u32([0, 0])))
+        out = b.up(np.full(q.shape, GUARD, np.uint16))
+        size = rt.tree_attention_workspace(cache, batch, heads)
+        rt.tree_attention(cache, batch, 0, heads, b.up(q), out, b.alloc(size), size,
+                          visible=b.up(np.array(masks, np.uint64)))
+        rt.synchronize()
+        got = values(rt.download(out, q.size, np.uint16).reshape(q.shape), dtype)
+        assert int(rt.download(status, 1, np.uint32)[0]) == 1
+    assert np.isnan(got[:nodes]).all(), np.argwhere(~np.isnan(got[:nodes]))[:4]
+    assert not got[nodes + 2].any()
+    for h in range(heads):
+        seen = np.array([[m >> j & 1 for j in range(5)] for m in masks[nodes:]], bool)
+        want, tol = attend(values(q[nodes:, h], dtype), values(pool_k[0, 4, h // 2, :5], dtype),
+                           values(pool_v[0, 4, h // 2, :5], dtype), seen, d ** -0.5, dtype)
+        check(got[nodes:, h], want, tol, f"head {h}")

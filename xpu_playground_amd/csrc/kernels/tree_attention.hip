@@ -354,7 +354,8 @@ template <int DT, int D, int R> XPU_DEVICE void tree_attention(const TreeArgs &a
     const uint32_t dim = wave * 2u * kMine + 4u * hh;
     if (in >= rows_in) continue;
     if (place.chunks == 1) {
-      const bool empty = s.context == 0 && a.visible && sees[r] == 0 && !bad;
+      // (the sum has the NaN of every wavefront that met a missing page)
+      const bool empty = s.context == 0 && a.visible && sees[r] == 0 && sum == 0.0f;
       const float by = empty ? 0.0f : 1.0f / sum;
       uint16_t *to = a.out + (s.first + row / group) * a.out_stride + (kvh * group + row % group) * D + dim;
 #pragma unroll
