@@ -101,11 +101,11 @@ template <int D> XPU_DEVICE void keep(const KeepArgs &a) {
     for (uint32_t i = 0; i < kLoads; ++i) {
       const uint32_t j = row + i * kRpi + lane / kCpr;
       const uint32_t node = a.kept[lo + (j < count ? j : 0u)];
-      const bool moves = j < count && node != j, exists = node < hi - lo && node < 64u;
+      const bool real = j < count, moves = real && node != j, exists = node < hi - lo && node < 64u;
       const uint64_t from = element(exists ? node : 0u), at = element(j);
       const bool fine = exists && from != kNowhere && at != kNowhere;
       to[i] = moves && fine && part < parts ? at : kNowhere;
-      odd |= moves && !fine;
+      odd |= real && !fine;  // also a row that stays where it is
       held[i] = *reinterpret_cast<const u32x4 *>(pool + (to[i] != kNowhere ? from : 0u));
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
