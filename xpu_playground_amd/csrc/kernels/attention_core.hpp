@@ -35,6 +35,7 @@ using dma::lds_s16x4;
 typedef uint32_t u32x8 __attribute__((ext_vector_type(8)));
 
 constexpr float kLazy = 8.0f;  // rescale when the maximum grows by more, in powers of two
+constexpr float kFar = 0x1p20f;  // a float holds powers of two up to here to 2^-4
 
 // Physical chunk = chunk ^ swizzle(row).
 template <int D> XPU_DEVICE uint32_t k_swz(uint32_t row) {
@@ -92,7 +93,8 @@ template <int DT, int D, int R> struct Rows {
   static constexpr uint32_t kRow = 2u * D;  // bytes of a key row
   u32x4 q[R][kKs];
   f32x16 o[R][kDt];
-  float m[R], sum[R];
+  float m[R], sum[R], shift[R];
+  float limit[R];  // wave-uniform: kLazy, or -inf where a reference is too large for its product with c (settle)
   uint32_t ka[kKs], va[kDt];  // the lane's LDS addresses in a K and a V tile at `base`
 
   // base: the LDS address that the tiles' offsets (kb, vb below) count from
@@ -101,7 +103,8 @@ template <int DT, int D, int R> struct Rows {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       m[r] = -__builtin_inff();
-      sum[r] = 0.0f;
+      sum[r] = shift[r] = 0.0f;
+      limit[r] = kLazy;
 #pragma unroll
       for (int dt = 0; dt < kDt; ++dt)
 #pragma unroll
@@ -187,39 +190,54 @@ template <int DT, int D, int R> struct Rows {
     return fmaxf(top, xor32_f(top));  // the query's other half-wave
   }
   // Moves the reference where `top` passes it by more than kLazy. c = scale
-  // log2 e > 0.
-  XPU_DEVICE void settle(int r, float top, float c) {
-    const float ninf = -__builtin_inff();
-    const bool grow = (top - m[r]) * c > kLazy;  // m = -inf: any finite score
-    if (__builtin_amdgcn_ballot_w64(grow)) {
-      const float now = grow ? top : m[r];
-      const float a = m[r] == ninf ? 0.0f : __builtin_amdgcn_exp2f((m[r] - now) * c);
-      sum[r] *= a;
+  // log2 e > 0. The exponents are s c + shift in one FMA each; shift = -m c is
+  // off by up to 2^-24 of itself, for all keys alike, which cancels in the
+  // result as long as p stays in the storage type's range. Where a reference
+  // passes kFar, the tile's scores become their differences from m, which are
+  // exact enough at any size, and shift is 0: `limit` then lets every tile in
+  // here, so that the others pay nothing for it.
+  template <int T> XPU_DEVICE void settle(int r, f32x16 (&s)[T], float top, float c) {
+    const float ninf = -__builtin_inff(), by = (top - m[r]) * c;  // m = -inf: inf for any finite score
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(by >= limit[r]) != 0, 0)) {  // >=: by may be -inf
+      const bool grow = by > kLazy;
+      if (__builtin_amdgcn_ballot_w64(grow)) {
+        const float now = grow ? top : m[r];
+        const float a = m[r] == ninf ? 0.0f : __builtin_amdgcn_exp2f((m[r] - now) * c);
+        sum[r] *= a;
 #pragma unroll
-      for (int dt = 0; dt < kDt; ++dt)
+        for (int dt = 0; dt < kDt; ++dt)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[r][dt][i] *= a;
-      m[r] = now;
+          for (int i = 0; i < 16; ++i) o[r][dt][i] *= a;
+        m[r] = now;
+        if (__builtin_amdgcn_ballot_w64(now != ninf && __builtin_fabsf(now * c) > kFar)) limit[r] = ninf;
+        shift[r] = now == ninf || limit[r] == ninf ? 0.0f : -now * c;  // no score yet: every p is 0
+      }
+      if (limit[r] == ninf) {
+        const float from = m[r] == ninf ? 0.0f : m[r];
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[t][i] -= from;
+      }
     }
   }
   // p of the tile packed as the MFMA takes it, word i of pk[t] for registers 2 i
   // and 2 i + 1, and their sum.
   template <int T> XPU_DEVICE void powers(int r, const f32x16 (&s)[T], float c, u32x8 (&pk)[T]) {
-    const float shift = m[r] == -__builtin_inff() ? 0.0f : -m[r] * c;  // no score yet: every p is 0
     float part = 0.0f;
 #pragma unroll
     for (int t = 0; t < T; ++t)
 #pragma unroll
       for (int i = 0; i < 16; i += 2) {
-        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], c, shift));
-        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i + 1], c, shift));
+        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], c, shift[r]));
+        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i + 1], c, shift[r]));
         pk[t][i / 2] = dma::cvt_pack<DT>(e0, e1);
         part = add_pair<DT>(pk[t][i / 2], part);
       }
     sum[r] += part;
   }
-  template <int T> XPU_DEVICE void softmax(int r, const f32x16 (&s)[T], float c, u32x8 (&pk)[T]) {
-    settle(r, largest<T>(s), c);
+  template <int T> XPU_DEVICE void softmax(int r, f32x16 (&s)[T], float c, u32x8 (&pk)[T]) {
+    settle<T>(r, s, largest<T>(s), c);
     powers<T>(r, s, c, pk);
   }
 

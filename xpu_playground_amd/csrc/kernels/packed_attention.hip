@@ -200,7 +200,7 @@ template <int DT, int D> XPU_DEVICE void packed_attention(const PackedArgs &a) {
       __syncthreads();
       issue(tile + stage_of + 1, false, true);
       issue(tile + stage_of + 2, true, false);
-      rows.settle(0, top, a.scale_log2e);
+      rows.template settle<2>(0, s, top, a.scale_log2e);
       rows.scores_powers(kb, next, s, a.scale_log2e, pk[0]);
       top = rows.values_largest(vb, pk[0], next);
     };
@@ -212,7 +212,7 @@ template <int DT, int D> XPU_DEVICE void packed_attention(const PackedArgs &a) {
     wait_vmcnt<0>();
     __syncthreads();
     issue(tile + 1, whole == 1, true);
-    rows.settle(0, top, a.scale_log2e);
+    rows.template settle<2>(0, s0, top, a.scale_log2e);
     rows.template powers<2>(0, s0, a.scale_log2e, pk[0]);
     rows.template values<2>(kTile, pk);
     ++tile;
