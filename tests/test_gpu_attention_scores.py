@@ -102,3 +102,39 @@ def test_large_scores(rt, attention, d, sign, dtype, a, b, step, scales):
             assert np.array_equal(scores, scores.astype(np.float32))
             want, tol = softmax(scores, vf[:, h], float(np.float32(scale)), dtype)
             check(got[:, h], want, tol, f"scale {scale} head {h}")
+
+
+def far_below(shift, d, n, every):
+    """Keys whose score is `shift` below that of one key in `every`, which has the value 0."""
+    k, v = np.zeros((n, 1, d)), np.full((n, 1, d), 1024.0)
+    top = np.arange(n) % every == 5 % every
+    k[~top, 0, 1], v[top] = -shift, 0
+    return k, v, top
+
+
+@pytest.mark.parametrize("attention", [prompt, tree])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("shift", [9.0, 10.4, 13.0, 16.0, 17.25, 18.0])
+@pytest.mark.parametrize("n,every", [(700, 32), (100000, 100000)])
+def test_many_keys_far_below_the_largest_in_fp16(rt, attention, d, shift, n, every):
+    """The probabilities e^-9 .. e^-18 of most keys are 2^-13 .. 2^-26, around
+    the end of fp16's normal range and far into the range below it. The result
+    is their part of the sum, which is all that the bound goes by. p is scaled by
+    2^7 before it is rounded, so its absolute rounding below the normal range is
+    2^-25 / 2^7 = 2^-32 of the largest."""
+    dtype = xpu.FP16
+    k, v, top = far_below(shift, d, n, every)
+    q = np.zeros((1, 1, d))
+    q[0, 0, 1] = 1
+    q, k, v = codes(q, dtype), codes(k, dtype), codes(v, dtype)
+    print(f"far below {attention.__name__} d {d} shift {shift} keys {n}", flush=True)
+    got = values(attention(rt, q, k, v, dtype, 1.0), dtype)[0, 0]
+    shift = -float(values(k, dtype).min())  # as the type holds it: 10.4 is 10.3984375
+    low, high = (n - top.sum()) * np.exp(-shift), top.sum()
+    o, u = 1024 * low / (low + high), HALF_STEP[dtype]
+    # e: exp2 and its argument; each key's rounding (u, and 2^-32 where e^-shift 2^7
+    # is below 2^-14); sums of n terms in FP32; the result's rounding
+    e = shift * 2.0 ** -22 + 2.0 ** -19
+    size = u + (2.0 ** -32 / np.exp(-shift) if np.exp(-shift) < 2.0 ** -21 else 0.0)
+    tol = o * (size + 2 * e + n * 2.0 ** -24 * 2 + u) * (1 + 4 * u) + TINY[dtype]
+    assert (np.abs(got - o) <= tol).all(), (got[0], o, tol)

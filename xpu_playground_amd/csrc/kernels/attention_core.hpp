@@ -8,7 +8,8 @@
 //                    the FP32 sum of p, and the FP32 output columns; m moves
 //                    (and sum and output are rescaled) only when a score
 //                    passes it by more than 8 in the exponent, so p <= 256
-//                    and rescales are rare after the first tiles
+//                    and rescales are rare after the first tiles; in fp16 all
+//                    of it is 2^7 times as large (kLift)
 //   O^T += V^T P^T   B operand: the lane's own p, rounded to the storage type
 //                    where the MFMA reads it (the only rounding between the
 //                    inputs and the result's own), A operand: V^T by the
@@ -35,6 +36,12 @@ using dma::lds_s16x4;
 typedef uint32_t u32x8 __attribute__((ext_vector_type(8)));
 
 constexpr float kLazy = 8.0f;  // rescale when the maximum grows by more, in powers of two
+// p is formed 2^kLift times as large: fp16 then holds it to a full relative step
+// from 2^-21 of the largest on, and to 2^-32 below (without: 2^-14 and 2^-25, and
+// the many small ones of a long context came out up to 6% off), and with kLazy it
+// stays below 2^15. The factor is in the sums and in the output alike, in every
+// partial result, and cancels. bf16 has the exponents of FP32.
+template <int DT> constexpr float kLift = DT == kFp16 ? 7.0f : 0.0f;
 constexpr float kFar = 0x1p20f;  // a float holds powers of two up to here to 2^-4
 
 // Physical chunk = chunk ^ swizzle(row).
@@ -210,7 +217,7 @@ template <int DT, int D, int R> struct Rows {
           for (int i = 0; i < 16; ++i) o[r][dt][i] *= a;
         m[r] = now;
         if (__builtin_amdgcn_ballot_w64(now != ninf && __builtin_fabsf(now * c) > kFar)) limit[r] = ninf;
-        shift[r] = now == ninf || limit[r] == ninf ? 0.0f : -now * c;  // no score yet: every p is 0
+        shift[r] = limit[r] == ninf ? kLift<DT> : now == ninf ? 0.0f : kLift<DT> - now * c;
       }
       if (limit[r] == ninf) {
         const float from = m[r] == ninf ? 0.0f : m[r];
