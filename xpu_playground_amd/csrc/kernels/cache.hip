@@ -14,16 +14,32 @@
 namespace xpu {
 namespace cache {
 
-// The sequence that holds row `row` of the batch, or -1 (behind the last
-// one, or starts that do not ascend). The starts are counted 64 at a time.
-XPU_DEVICE int32_t sequence_of_row(const BatchArgs &b, uint32_t row) {
-  uint32_t s = 0;
-  for (uint32_t at = 1; at <= b.n_seqs; at += 64) {
-    const uint32_t i = at + lane_id();
-    s += __builtin_popcountll(__builtin_amdgcn_ballot_w64(i <= b.n_seqs && b.starts[i] <= row));
+// The sequence that holds row `row` of the batch, and its first row; seq -1
+// for a row of none. 64 sequences at a time, a lane each, the next 64 on their
+// way; the first that has the row, whatever the starts of the others are.
+struct Holder {
+  int32_t seq;
+  uint32_t first;
+};
+XPU_DEVICE Holder holder_of(const BatchArgs &b, uint32_t row) {
+  uint32_t lo, hi, next_lo, next_hi;
+  auto load = [&](uint32_t at, uint32_t &l, uint32_t &h) {  // past the last: it again, behind itself
+    const uint32_t i = min(at + lane_id(), b.n_seqs - 1u);
+    l = b.starts[i];
+    h = b.starts[i + 1u];
+  };
+  load(0, lo, hi);
+  for (uint32_t at = 0;;) {
+    load(at + 64u, next_lo, next_hi);
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(lo <= row && row < hi && hi <= b.rows);
+    if (hit) {
+      const uint32_t l = __builtin_ctzll(hit);
+      return {static_cast<int32_t>(at + l), static_cast<uint32_t>(__builtin_amdgcn_readlane(lo, l))};
+    }
+    if ((at += 64u) >= b.n_seqs) return {-1, 0};
+    lo = next_lo;
+    hi = next_hi;
   }
-  if (s >= b.n_seqs || b.starts[s] > row || b.starts[s + 1] <= row || b.starts[s + 1] > b.rows) return -1;
-  return static_cast<int32_t>(__builtin_amdgcn_readfirstlane(s));
 }
 
 XPU_DEVICE void report(const PoolArgs &p) {
@@ -36,9 +52,10 @@ template <int D> XPU_DEVICE void append(const AppendArgs &a) {
   const uint32_t lane = lane_id(), waves = gridDim.x * 4u, chunks = a.pool.kv_heads * kCpr;
   for (uint32_t row = blockIdx.x * 4u + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); row < a.batch.rows;
        row += waves) {
-    const int32_t seq = sequence_of_row(a.batch, row);
-    if (seq < 0) continue;
-    const uint64_t pos = static_cast<uint64_t>(a.batch.context[seq]) + (row - a.batch.starts[seq]);
+    const Holder holder = holder_of(a.batch, row);
+    if (holder.seq < 0) continue;
+    const uint32_t seq = static_cast<uint32_t>(holder.seq);
+    const uint64_t pos = static_cast<uint64_t>(a.batch.context[seq]) + (row - holder.first);
     const uint64_t at = element_of(a.pool, a.batch.tables + static_cast<uint64_t>(seq) * a.batch.table_pitch, a.batch.table_pitch, pos, D);
     if (at == kNowhere) {
       report(a.pool);
