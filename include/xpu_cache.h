@@ -127,7 +127,8 @@ int xpu_cache_copy(xpu_runtime *rt, const xpu_cache *cache, const uint32_t *src,
  * keys the first keys are an earlier part of the prompt. k_starts NULL: the
  * same rows. A query that sees no key gives zeros. Rows that belong to no
  * sequence are left as they are; so are those of a sequence whose starts do
- * not ascend or pass the rows. */
+ * not ascend or pass the rows; rows that several sequences claim get any one's
+ * result or none. */
 typedef struct {
   int32_t dtype;
   uint32_t heads, kv_heads, head_dim; /* head_dim 64 or 128 */

@@ -65,25 +65,26 @@ XPU_DEVICE Work heaviest_first(const PackedArgs &a, uint32_t shift, uint32_t ran
   return {static_cast<int32_t>(l), place << shift, of(w.q_lo), of(w.q_hi), of(w.k_lo), of(w.k_hi)};
 }
 
-// Work item `slot` of any number of sequences, the last first: sequence s has
-// the slots from (starts[s] >> shift) + s on, at least as many as it has tiles,
-// and known without a sum over the sequences.
+// Work item `slot` of any number of sequences, the last first: the tiles are
+// numbered sequence by sequence, 64 at a time, the next 64 on their way.
 XPU_DEVICE Work by_slot(const PackedArgs &a, uint32_t shift, uint32_t slot) {
-  int32_t s = -1;
-  for (uint32_t at = 0; at < a.n_seqs; at += 64) {
-    const uint32_t i = at + lane_id();
-    const bool before = i < a.n_seqs && (a.q_starts[i] >> shift) + i <= slot;
-    s += __builtin_popcountll(__builtin_amdgcn_ballot_w64(before));
+  Work w{}, next{};
+  rows_of(a, min(lane_id(), a.n_seqs - 1u), w);
+  uint32_t before = 0;
+  for (uint32_t at = 0;;) {
+    rows_of(a, min(at + 64u + lane_id(), a.n_seqs - 1u), next);
+    const uint32_t tiles = at + lane_id() < a.n_seqs ? (w.q_hi - w.q_lo + (1u << shift) - 1u) >> shift : 0u;
+    const uint32_t upto = sum_upto(tiles), first = before + upto - tiles;
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(slot >= first && slot - first < tiles);
+    if (hit) {
+      const uint32_t l = __builtin_ctzll(hit);
+      auto of = [&](uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(v, l)); };
+      return {static_cast<int32_t>(at + l), (slot - of(first)) << shift, of(w.q_lo), of(w.q_hi), of(w.k_lo), of(w.k_hi)};
+    }
+    if ((at += 64u) >= a.n_seqs) return {-1, 0, 0, 0, 0, 0};
+    before += static_cast<uint32_t>(__builtin_amdgcn_readlane(upto, 63));
+    w = next;
   }
-  Work w{};
-  w.seq = __builtin_amdgcn_readfirstlane(s);
-  if (s < 0) return w;
-  rows_of(a, static_cast<uint32_t>(w.seq), w);
-  for (uint32_t *v : {&w.q_lo, &w.q_hi, &w.k_lo, &w.k_hi}) *v = __builtin_amdgcn_readfirstlane(*v);
-  const uint32_t base = (w.q_lo >> shift) + static_cast<uint32_t>(w.seq);
-  if (base > slot || (slot - base) << shift >= w.q_hi - w.q_lo) w.seq = -1;
-  w.first_q = (slot - base) << shift;
-  return w;
 }
 
 template <int DT, int D> XPU_DEVICE void packed_attention(const PackedArgs &a) {
