@@ -115,6 +115,51 @@ int launch(xpu_runtime *rt, const std::string &kernel, uint64_t grid, const A &a
   return rt->launch(*k, static_cast<uint32_t>(grid), grid_y, block, 0, list, more ? 2 : 1);
 }
 
+// Up to n ids of pages 0 .. pool - 1: a bit for each page of a pool that is not
+// large beside n, else open addressing in at least four times n places, so that
+// few pairs cost what they cost whatever the pool is. The host's part of a call:
+// 4 pairs in 1000000 pages 2.7 us by addressing, 13 by bits (in 64 pages 2.7);
+// 8192 pairs in 1000000 pages 44 and 29, in 100000 pages 53 and 21.
+class Ids {
+ public:
+  Ids(uint32_t n, uint32_t pool) {
+    if (pool / 256 < n) {
+      bits_.assign(pool / 64 + 1, 0);
+      return;
+    }
+    while ((1ull << (64 - shift_)) < 4ull * n) --shift_;
+    places_.assign(1ull << (64 - shift_), kNone);
+  }
+  // whether `id` was not there yet
+  bool add(uint32_t id) {
+    if (!bits_.empty()) {
+      uint64_t &word = bits_[id / 64];
+      const uint64_t bit = 1ull << id % 64;
+      const bool fresh = !(word & bit);
+      word |= bit;
+      return fresh;
+    }
+    uint32_t &at = places_[find(id)];
+    const bool fresh = at == kNone;
+    at = id;
+    return fresh;
+  }
+  bool has(uint32_t id) const {
+    return bits_.empty() ? places_[find(id)] == id : bits_[id / 64] >> id % 64 & 1;
+  }
+
+ private:
+  static constexpr uint32_t kNone = ~0u;  // no page: there are 2^32 - 1 at most
+  uint64_t find(uint32_t id) const {
+    uint64_t at = id * 0x9e3779b97f4a7c15ull >> shift_;  // 2^64 / the golden ratio: the top bits spread
+    while (places_[at] != kNone && places_[at] != id) at = (at + 1) & (places_.size() - 1);
+    return at;
+  }
+  int shift_ = 63;
+  std::vector<uint64_t> bits_;
+  std::vector<uint32_t> places_;
+};
+
 const char *type_name(int32_t dtype) { return dtype == XPU_DTYPE_FP16 ? "fp16" : "bf16"; }
 
 // How a tree attention call is cut (kernels/tree_attention.hip). Every rule
@@ -284,17 +329,14 @@ int xpu_cache_copy(xpu_runtime *rt, const xpu_cache *cache, const uint32_t *src,
     if (int rc = check_cache(name, cache, true)) return rc;
     if (!n) return check_runtime(name, rt);
     if (!src || !dst) return invalid(name, "null argument");
-    // 1: copied from, 2: copied to
-    std::vector<uint8_t> seen(cache->n_pages, 0);
+    Ids to(n, cache->n_pages);
     for (uint32_t i = 0; i < n; ++i) {
       if (src[i] >= cache->n_pages || dst[i] >= cache->n_pages)
         return invalid(name, "page " + std::to_string(std::max(src[i], dst[i])) + " does not exist");
-      seen[src[i]] |= 1;
-      if (seen[dst[i]] & 2) return invalid(name, "page " + std::to_string(dst[i]) + " is copied to twice");
-      seen[dst[i]] |= 2;
+      if (!to.add(dst[i])) return invalid(name, "page " + std::to_string(dst[i]) + " is copied to twice");
     }
     for (uint32_t i = 0; i < n; ++i)
-      if (seen[dst[i]] == 3) return invalid(name, "page " + std::to_string(dst[i]) + " is copied to and from");
+      if (to.has(src[i])) return invalid(name, "page " + std::to_string(src[i]) + " is copied to and from");
     if (int rc = check_runtime(name, rt)) return rc;
     const uint32_t chunks = cache->kv_heads * cache->page_size * cache->head_dim / 8;
     // the pairs travel as kernel arguments, so many at a time
