@@ -87,7 +87,8 @@ int xpu_cache_append(xpu_runtime *rt, const xpu_cache *cache, const xpu_batch *b
  * whatever they hold, NaN and infinities included.
  *   out[row][head] = softmax(scale * q . k) v,  head h on kv head h / (heads / kv_heads)
  * q and out: [rows][heads][head_dim] in the cache's type, rows q_stride and
- * out_stride elements apart; out must not overlap q. FP32 scores, softmax and
+ * out_stride elements apart; out must not overlap q (columns of one buffer, of
+ * one stride, do not). FP32 scores, softmax and
  * sums; the probabilities are rounded to the cache's type for the product
  * with V. scale > 0. A page id past n_pages, a context past the table or more
  * than 64 nodes under `visible` makes the rows of that sequence NaN and sets
@@ -141,7 +142,7 @@ typedef struct {
 /* out[row][head] = softmax(scale * q . k) v as xpu_tree_attention, causal
  * within each sequence. q, out: [q_rows][heads][head_dim]; k, v: [k_rows][
  * kv_heads][head_dim]. out may be q itself with its stride; otherwise it must
- * not overlap an input. */
+ * not overlap an input (columns of one buffer, of one stride, do not). */
 int xpu_prompt_attention(xpu_runtime *rt, const xpu_packed *packed, const void *q, const void *k, const void *v,
                          void *out);
 

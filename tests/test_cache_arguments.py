@@ -1,0 +1,42 @@
+"""Arguments of the paged cache's calls at the border of what is refused, on
+the host: a null runtime is the last thing that a call looks at."""
+import pytest
+
+from test_cache_refusals import A, INVALID, batch, packed, prompt, tree
+
+Q = 6 * A  # 10 rows of 4 heads x 64: 512 bytes each
+
+
+@pytest.mark.parametrize("stride,columns", [  # elements
+    (512, 256), (512, -256), (528, 256), (528, 264), (528, -264), (528, -272), (1024, 256), (1024, 768), (1024, -512)])
+def test_out_may_be_other_columns_of_the_buffer_that_holds_q(stride, columns):
+    """Rows the same stride apart that share no byte do not overlap, on either
+    side of q and whole rows away from it too."""
+    for rows_away in (0, 1, -1, 3):
+        at = Q + 2 * columns + 2 * stride * rows_away
+        for rc, text in (tree(q_stride=stride, out=at, out_stride=stride),
+                         prompt(packed(q_stride=stride, out_stride=stride), q=Q, out=at)):
+            assert rc == INVALID and text.endswith("null runtime"), text
+
+
+@pytest.mark.parametrize("stride", [512, 528])
+@pytest.mark.parametrize("columns", [8, 248, -8, -248, 0, 280])
+def test_out_that_shares_columns_with_q_is_refused(stride, columns):
+    for rows_away in (0, 1, -2, 9 if columns < 256 else 8):  # behind q's last row there is none to share with
+        at = Q + 2 * columns + 2 * stride * rows_away
+        rc, text = tree(q_stride=stride, out=at, out_stride=stride)
+        assert rc == INVALID and "overlap" in text, text
+        if columns or rows_away:
+            rc, text = prompt(packed(q_stride=stride, out_stride=stride), q=Q, out=at)
+            assert rc == INVALID and "overlap" in text, text
+    # past q's last row, or before its first, there is nothing to share
+    for rows_away in (10, -10):
+        rc, text = tree(q_stride=stride, out=Q + 2 * stride * rows_away, out_stride=stride)
+        assert text.endswith("null runtime"), text
+
+
+def test_other_strides_that_cross_are_refused():
+    rc, text = tree(q_stride=512, out=Q + 512, out_stride=520)
+    assert rc == INVALID and "overlap" in text
+    rc, text = tree(b=batch(rows=1), q_stride=512, out=Q + 512, out_stride=520)
+    assert text.endswith("null runtime"), text

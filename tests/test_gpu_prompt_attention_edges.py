@@ -3,8 +3,8 @@ import numpy as np
 import pytest
 
 import xpu_playground_amd as xpu
-from cache_util import GUARD, attend, check, normal, u32, values
-from test_gpu_prompt_attention import launch
+from cache_util import GUARD, Buffers, attend, check, normal, u32, values
+from test_gpu_prompt_attention import expected, launch
 
 pytestmark = pytest.mark.gpu
 
@@ -57,3 +57,25 @@ def test_starts_that_do_not_fit_among_many(rt, heads, kv, n, what):
             check(got[a:b, h][one], want[one], tol[one], f"sequence {s} head {h}")
         checked += int(one.sum())
     assert checked > rows // 4
+
+
+@pytest.mark.parametrize("dtype", [xpu.BF16, xpu.FP16])
+@pytest.mark.parametrize("before", [False, True])
+def test_out_beside_q_in_one_buffer(rt, dtype, before):
+    """q and out as columns of one buffer, in either order."""
+    heads, d, n = 4, 64, 150
+    x = np.full((n, 2 * heads * d + 8), GUARD, np.uint16)
+    at_q, at_out = (heads * d + 8, 0) if before else (0, heads * d + 8)
+    q, k, v = normal((n, heads, d), 1, dtype), normal((n, 2, d), 2, dtype), normal((n, 2, d), 3, dtype)
+    x[:, at_q:at_q + heads * d] = q.reshape(n, -1)
+    starts = u32([1, 100, 149])
+    want, tol = expected(q, k, v, starts, starts, d ** -0.5, dtype, np.full(q.shape, GUARD, np.uint16))
+    with Buffers(rt) as b:
+        at = b.up(x)
+        p = xpu.Packed(dtype, heads, 2, d, 2, n, b.up(starts), q_stride=x.shape[1], out_stride=x.shape[1])
+        rt.prompt_attention(p, at + 2 * at_q, b.up(k), b.up(v), at + 2 * at_out)
+        rt.synchronize()
+        y = rt.download(at, x.size, np.uint16).reshape(x.shape)
+    check(values(y[:, at_out:at_out + heads * d].reshape(q.shape), dtype), want, tol)
+    y[:, at_out:at_out + heads * d] = GUARD
+    assert np.array_equal(y, x)

@@ -5,6 +5,7 @@ import pytest
 
 import xpu_playground_amd as xpu
 from cache_util import GUARD, Buffers, attend, check, normal, u32, values
+from test_gpu_tree_attention import Case
 
 pytestmark = pytest.mark.gpu
 
@@ -44,3 +45,26 @@ def test_rows_that_see_nothing_of_missing_pages(rt, dtype, d, nodes, missing):
         want, tol = attend(values(q[nodes:, h], dtype), values(pool_k[0, 4, h // 2, :5], dtype),
                            values(pool_v[0, 4, h // 2, :5], dtype), seen, d ** -0.5, dtype)
         check(got[nodes:, h], want, tol, f"head {h}")
+
+
+@pytest.mark.parametrize("dtype", [xpu.BF16, xpu.FP16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("before", [False, True])
+def test_out_beside_q_in_one_buffer(rt, dtype, d, before):
+    """q and out as columns of one buffer, in either order, with a cut and an
+    uncut sequence; nothing but the sequences' columns of out changes."""
+    case = Case([3, 40], [2000, 20], 4, 2, d, 16, dtype, 31, first=1)
+    want, tol = case.expected(d ** -0.5)
+    width = case.heads * d
+    x = np.full((case.rows, 2 * width + 8), GUARD, np.uint16)
+    at_q, at_out = (width + 8, 0) if before else (0, width + 8)
+    x[:, at_q:at_q + width] = case.q.reshape(case.rows, -1)
+    with Buffers(rt) as b:
+        args, at = case.device(b), b.up(x)
+        args.update(q=at + 2 * at_q, out=at + 2 * at_out, q_stride=x.shape[1], out_stride=x.shape[1])
+        rt.tree_attention(**args)
+        rt.synchronize()
+        y = rt.download(at, x.size, np.uint16).reshape(x.shape)
+    check(values(y[:, at_out:at_out + width].reshape(case.out.shape), dtype), want, tol)
+    y[:, at_out:at_out + width] = GUARD
+    assert np.array_equal(y, x)

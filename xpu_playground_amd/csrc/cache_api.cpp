@@ -28,6 +28,16 @@ bool overlap(const void *a, uint64_t a_bytes, const void *b, uint64_t b_bytes) {
 // The bytes that `rows` rows of `width` elements span.
 uint64_t span(uint64_t rows, uint64_t stride, uint64_t width) { return rows ? ((rows - 1) * stride + width) * 2 : 0; }
 
+// Whether rows of `width` elements at a and at b share a byte. Rows the same
+// stride apart may lie side by side, as columns of one buffer.
+bool rows_overlap(uint64_t rows, uint64_t width, const void *a, uint64_t a_stride, const void *b, uint64_t b_stride) {
+  if (!overlap(a, span(rows, a_stride, width), b, span(rows, b_stride, width))) return false;
+  if (a_stride != b_stride) return true;
+  const uint64_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b), stride = 2 * a_stride;
+  const uint64_t apart = (x < y ? y - x : x - y) % stride;
+  return apart < 2 * width || stride - apart < 2 * width;
+}
+
 // A launch's threads have to fit 32 bits.
 constexpr uint64_t kMostBlocks = (1ull << 24) - 1;
 
@@ -267,7 +277,7 @@ int xpu_tree_attention(xpu_runtime *rt, const xpu_cache *cache, const xpu_batch 
     if (int rc = check_rows(name, "q", q, q_stride, width)) return rc;
     if (int rc = check_rows(name, "out", out, out_stride, width)) return rc;
     if (!aligned(visible, 8)) return invalid(name, "visible must be 8-byte aligned");
-    if (overlap(q, span(batch->rows, q_stride, width), out, span(batch->rows, out_stride, width)))
+    if (rows_overlap(batch->rows, width, q, q_stride, out, out_stride))
       return invalid(name, "out must not overlap q");
     if (static_cast<uint64_t>(batch->rows) * heads >= (1ull << 26)) return invalid(name, "too many rows");
     if (int rc = check_runtime(name, rt)) return rc;
@@ -376,9 +386,8 @@ int xpu_prompt_attention(xpu_runtime *rt, const xpu_packed *p, const void *q, co
       if (int rc = check_rows(name, "k", k, p->k_stride, k_width)) return rc;
       if (int rc = check_rows(name, "v", v, p->v_stride, k_width)) return rc;
     }
-    const uint64_t out_bytes = span(p->q_rows, p->out_stride, q_width);
     if (!(out == q && p->out_stride == p->q_stride) &&
-        overlap(q, span(p->q_rows, p->q_stride, q_width), out, out_bytes))
+        rows_overlap(p->q_rows, q_width, q, p->q_stride, out, p->out_stride))
       return invalid(name, "out must be q or not overlap it");
     if (int rc = check_runtime(name, rt)) return rc;
     xpu::PackedArgs a{};
