@@ -1,8 +1,11 @@
 """Arguments of the paged cache's calls at the border of what is refused, on
 the host: a null runtime is the last thing that a call looks at."""
+import numpy as np
 import pytest
 
+import xpu_playground_amd as xpu
 from test_cache_refusals import A, INVALID, batch, packed, prompt, tree
+from xpu_playground_amd.cache import Pages
 
 Q = 6 * A  # 10 rows of 4 heads x 64: 512 bytes each
 
@@ -40,3 +43,30 @@ def test_other_strides_that_cross_are_refused():
     assert rc == INVALID and "overlap" in text
     rc, text = tree(b=batch(rows=1), q_stride=512, out=Q + 512, out_stride=520)
     assert text.endswith("null runtime"), text
+
+
+WIDE = [1 << 32, (1 << 32) + 4, -1, -(1 << 32)]
+
+
+@pytest.mark.parametrize("n", WIDE)
+def test_page_counts_that_32_bits_do_not_hold(n):
+    """Cut to 32 bits, 2^32 would be nothing, and take() would return what its
+    array held before."""
+    with pytest.raises(ValueError, match="32"):
+        Pages(n)
+    p = Pages(8)
+    p.take(3)
+    for call in (p.take, p.holders):
+        with pytest.raises(ValueError, match="32"):
+            call(n)
+    assert p.free == 5 and [p.holders(i) for i in range(4)] == [1, 1, 1, 0]
+
+
+def test_page_counts_that_are_no_integers():
+    for n in (1.0, "1", None):
+        with pytest.raises(TypeError):
+            Pages(n)
+        p = Pages(2)
+        with pytest.raises(TypeError):
+            p.take(n)
+    assert list(Pages(np.int64(3)).take(np.uint8(2))) == [0, 1]

@@ -7,6 +7,7 @@ tree_attention.
 from __future__ import annotations
 
 import ctypes
+import operator
 from ctypes import c_uint32, c_void_p
 
 import numpy as np
@@ -14,12 +15,19 @@ import numpy as np
 from . import check, library, page_ids
 
 
+def _u32(n) -> int:
+    n = operator.index(n)
+    if not 0 <= n <= 0xFFFFFFFF:
+        raise ValueError(f"{n} is no unsigned 32-bit integer")
+    return n
+
+
 class Pages:
     """Counts the holders of n pages."""
 
     def __init__(self, n_pages: int):
         self.lib = library()
-        self.handle = None
+        self.handle, n_pages = None, _u32(n_pages)
         handle = c_void_p()
         check(self.lib.xpu_pages_create(n_pages, ctypes.byref(handle)))
         self.handle, self.n_pages = handle, n_pages
@@ -37,11 +45,12 @@ class Pages:
 
     def holders(self, page: int) -> int:
         v = c_uint32()
-        check(self.lib.xpu_pages_holders(self.handle, page, ctypes.byref(v)))
+        check(self.lib.xpu_pages_holders(self.handle, _u32(page), ctypes.byref(v)))
         return v.value
 
     def take(self, n: int) -> np.ndarray:
         """n free pages, lowest ids first."""
+        n = _u32(n)
         out = np.empty(min(n, self.n_pages), np.uint32)  # a larger n is refused before anything is written
         check(self.lib.xpu_pages_take(self.handle, n, out.ctypes.data))
         return out
