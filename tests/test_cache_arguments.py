@@ -70,3 +70,29 @@ def test_page_counts_that_are_no_integers():
         with pytest.raises(TypeError):
             p.take(n)
     assert list(Pages(np.int64(3)).take(np.uint8(2))) == [0, 1]
+
+
+@pytest.mark.parametrize("n", WIDE)
+def test_descriptions_that_their_fields_do_not_hold(n):
+    """A size past 32 bits is refused and not taken for what is left of it: a
+    Packed of 2^32 rows would be one of none, which does nothing."""
+    for make in (lambda: xpu.Packed(0, 4, 2, 64, 2, n, A), lambda: xpu.Packed(0, 4, 2, 64, n, 8, A),
+                 lambda: xpu.Packed(0, 4, 2, 64, 2, 8, A, k_rows=n), lambda: xpu.Batch(n, 4, 4, A, A, A),
+                 lambda: xpu.Batch(2, n, 4, A, A, A), lambda: xpu.Batch(2, 4, n, A, A, A),
+                 lambda: xpu.Batch(n_seqs=2, rows=4, table_pitch=n), lambda: xpu.Cache(0, n, 2, 64, 16, 8, A, A),
+                 lambda: xpu.Cache(0, 2, 2, 64, 16, n, A, A, layer_stride=1 << 20),
+                 lambda: xpu.Cache(0, 2, 2, 64, 16, 8, A, A, page_stride=(1 << 64) + 2048),
+                 lambda: xpu.Packed(0, 4, 2, 64, 2, 8, A, q_stride=-256)):
+        with pytest.raises(ValueError, match="bits"):
+            make()
+
+
+def test_descriptions_hold_what_they_were_given():
+    b = xpu.Batch(1, (1 << 31) - 1, np.uint32(7), A, A, None)
+    assert (b.n_seqs, b.rows, b.table_pitch, b.tables, b.context) == (1, (1 << 31) - 1, 7, A, None)
+    b = xpu.Batch(rows=5)
+    assert (b.n_seqs, b.rows, b.starts) == (0, 5, None)
+    c = xpu.Cache(-1, 4, 2, 64, 16, 0xFFFFFFFF, A, A, layer_stride=(1 << 64) - 8)
+    assert (c.dtype, c.n_pages, c.layer_stride, c.page_stride) == (-1, 0xFFFFFFFF, (1 << 64) - 8, 2048)
+    p = xpu.Packed(1, 4, 2, 64, 3, 0xFFFFFFFF, A, scale=2)
+    assert (p.q_rows, p.k_rows, p.scale, p.q_stride) == (0xFFFFFFFF, 0xFFFFFFFF, 2.0, 256)

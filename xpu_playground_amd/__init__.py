@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import weakref
 from array import array
 from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_size_t, c_uint32, c_uint64, c_void_p
@@ -71,6 +72,14 @@ def page_ids(ids):
     return np.ascontiguousarray(ids, dtype=np.uint32)
 
 
+def _fit(what: str, layout: struct.Struct, *values) -> None:
+    """Raises for integers that their fields do not hold; ctypes would cut them."""
+    try:
+        layout.pack(*values)
+    except struct.error as e:
+        raise ValueError(f"{what}: sizes have to fit the 32 or 64 bits of their fields: {e}") from None
+
+
 class Cache(ctypes.Structure):
     """xpu_cache (include/xpu_cache.h): the pages of a KV cache. k and v are
     device addresses; without strides the pools are [layers][n_pages]
@@ -89,13 +98,15 @@ class Cache(ctypes.Structure):
         ("v", c_void_p),
         ("status", c_void_p),
     ]
+    _sizes = struct.Struct("i5I2Q")
 
     def __init__(self, dtype, layers, kv_heads, head_dim, page_size, n_pages, k=None, v=None, status=None,
                  layer_stride=None, page_stride=None):
         page = kv_heads * page_size * head_dim
-        super().__init__(dtype, layers, kv_heads, head_dim, page_size, n_pages,
-                         n_pages * page if layer_stride is None else layer_stride,
-                         page if page_stride is None else page_stride, k, v, status)
+        sizes = (dtype, layers, kv_heads, head_dim, page_size, n_pages,
+                 n_pages * page if layer_stride is None else layer_stride, page if page_stride is None else page_stride)
+        _fit("Cache", self._sizes, *sizes)
+        super().__init__(*sizes, k, v, status)
 
 
 class Batch(ctypes.Structure):
@@ -110,6 +121,11 @@ class Batch(ctypes.Structure):
         ("starts", c_void_p),
         ("context", c_void_p),
     ]
+    _sizes = struct.Struct("3I")
+
+    def __init__(self, n_seqs=0, rows=0, table_pitch=0, tables=None, starts=None, context=None):
+        _fit("Batch", self._sizes, n_seqs, rows, table_pitch)
+        super().__init__(n_seqs, rows, table_pitch, tables, starts, context)
 
 
 class Packed(ctypes.Structure):
@@ -134,15 +150,17 @@ class Packed(ctypes.Structure):
         ("v_stride", c_uint64),
         ("out_stride", c_uint64),
     ]
+    _sizes = struct.Struct("i6I4Q")
 
     def __init__(self, dtype, heads, kv_heads, head_dim, n_seqs, q_rows, q_starts, k_rows=None, k_starts=None,
                  scale=None, q_stride=None, k_stride=None, v_stride=None, out_stride=None):
         def dense(stride, n):
             return n * head_dim if stride is None else stride
 
-        super().__init__(dtype, heads, kv_heads, head_dim, n_seqs, q_rows, q_rows if k_rows is None else k_rows,
-                         head_dim ** -0.5 if scale is None else scale, q_starts, k_starts, dense(q_stride, heads),
-                         dense(k_stride, kv_heads), dense(v_stride, kv_heads), dense(out_stride, heads))
+        sizes = (dtype, heads, kv_heads, head_dim, n_seqs, q_rows, q_rows if k_rows is None else k_rows)
+        strides = dense(q_stride, heads), dense(k_stride, kv_heads), dense(v_stride, kv_heads), dense(out_stride, heads)
+        _fit("Packed", self._sizes, *sizes, *strides)
+        super().__init__(*sizes, head_dim ** -0.5 if scale is None else scale, q_starts, k_starts, *strides)
 
 
 _lib = None
