@@ -96,3 +96,16 @@ def test_descriptions_hold_what_they_were_given():
     assert (c.dtype, c.n_pages, c.layer_stride, c.page_stride) == (-1, 0xFFFFFFFF, (1 << 64) - 8, 2048)
     p = xpu.Packed(1, 4, 2, 64, 3, 0xFFFFFFFF, A, scale=2)
     assert (p.q_rows, p.k_rows, p.scale, p.q_stride) == (0xFFFFFFFF, 0xFFFFFFFF, 2.0, 256)
+
+
+@pytest.mark.parametrize("ids", [b"\x01\0\0\0", bytearray(8), b""])
+def test_page_ids_are_no_bytes(ids):
+    """Four bytes were one id: what a program stores as bytes has to say how."""
+    with pytest.raises(ValueError, match="page ids"):
+        xpu.page_ids(ids)
+    p = Pages(4)
+    p.take(2)
+    with pytest.raises(ValueError, match="page ids"):
+        p.release(ids)
+    assert p.free == 2
+    assert list(xpu.page_ids(memoryview(np.array([3, 0xFFFFFFFF], np.uint32)))) == [3, 0xFFFFFFFF]

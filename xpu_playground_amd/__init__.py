@@ -60,6 +60,8 @@ def page_ids(ids):
 
     if not isinstance(ids, np.ndarray):
         try:
+            if isinstance(ids, (bytes, bytearray)):  # array takes these for its memory
+                raise TypeError("bytes")
             ids = array("I", ids)
             ids = np.frombuffer(ids, np.uint32) if ids else np.empty(0, np.uint32)
         except (TypeError, OverflowError) as e:
