@@ -42,10 +42,10 @@ int check_held(const xpu_pages *p, const uint32_t *ids, uint32_t n, const char *
 extern "C" {
 
 int xpu_pages_create(uint32_t n_pages, xpu_pages **out) {
-  if (!out) return set_error(XPU_ERR_INVALID, "xpu_pages_create: null output");
-  *out = nullptr;
-  if (!n_pages) return set_error(XPU_ERR_INVALID, "xpu_pages_create: n_pages must be positive");
   return guarded("xpu_pages_create", [&] {
+    if (!out) return set_error(XPU_ERR_INVALID, "xpu_pages_create: null output");
+    *out = nullptr;
+    if (!n_pages) return set_error(XPU_ERR_INVALID, "xpu_pages_create: n_pages must be positive");
     auto p = std::make_unique<xpu_pages>();
     p->holders.assign(n_pages, 0);
     std::vector<uint32_t> ids(n_pages);
@@ -59,16 +59,20 @@ int xpu_pages_create(uint32_t n_pages, xpu_pages **out) {
 void xpu_pages_destroy(xpu_pages *pages) { delete pages; }
 
 int xpu_pages_free_count(const xpu_pages *pages, uint32_t *count) {
-  if (!pages || !count) return set_error(XPU_ERR_INVALID, "xpu_pages_free_count: null argument");
-  *count = static_cast<uint32_t>(pages->free.size());
-  return XPU_OK;
+  return guarded("xpu_pages_free_count", [&] {
+    if (!pages || !count) return set_error(XPU_ERR_INVALID, "xpu_pages_free_count: null argument");
+    *count = static_cast<uint32_t>(pages->free.size());
+    return XPU_OK;
+  });
 }
 
 int xpu_pages_holders(const xpu_pages *pages, uint32_t id, uint32_t *count) {
-  if (!pages || !count) return set_error(XPU_ERR_INVALID, "xpu_pages_holders: null argument");
-  if (id >= pages->holders.size()) return set_error(XPU_ERR_INVALID, "xpu_pages_holders: no such page");
-  *count = pages->holders[id];
-  return XPU_OK;
+  return guarded("xpu_pages_holders", [&] {
+    if (!pages || !count) return set_error(XPU_ERR_INVALID, "xpu_pages_holders: null argument");
+    if (id >= pages->holders.size()) return set_error(XPU_ERR_INVALID, "xpu_pages_holders: no such page");
+    *count = pages->holders[id];
+    return XPU_OK;
+  });
 }
 
 int xpu_pages_take(xpu_pages *pages, uint32_t n, uint32_t *ids) {
@@ -132,8 +136,8 @@ int xpu_pages_own(xpu_pages *pages, uint32_t *ids, uint32_t n, uint32_t *src, ui
 }
 
 int xpu_pages_compact(xpu_pages *pages, uint32_t *src, uint32_t *dst, uint32_t *moves) {
-  if (!pages || !src || !dst || !moves) return set_error(XPU_ERR_INVALID, "xpu_pages_compact: null argument");
   return guarded("xpu_pages_compact", [&] {
+    if (!pages || !src || !dst || !moves) return set_error(XPU_ERR_INVALID, "xpu_pages_compact: null argument");
     const uint32_t n = static_cast<uint32_t>(pages->holders.size());
     const uint32_t used = n - static_cast<uint32_t>(pages->free.size());
     std::vector<uint32_t> ids;
@@ -155,9 +159,9 @@ int xpu_pages_compact(xpu_pages *pages, uint32_t *src, uint32_t *dst, uint32_t *
 }
 
 int xpu_pages_renumber(const uint32_t *src, const uint32_t *dst, uint32_t moves, uint32_t *ids, uint32_t n) {
-  if ((moves && (!src || !dst)) || (n && !ids))
-    return set_error(XPU_ERR_INVALID, "xpu_pages_renumber: null argument");
   return guarded("xpu_pages_renumber", [&] {
+    if ((moves && (!src || !dst)) || (n && !ids))
+      return set_error(XPU_ERR_INVALID, "xpu_pages_renumber: null argument");
     std::vector<std::pair<uint32_t, uint32_t>> map(moves);
     for (uint32_t i = 0; i < moves; ++i) map[i] = {src[i], dst[i]};
     std::sort(map.begin(), map.end());
