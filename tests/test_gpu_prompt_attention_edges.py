@@ -1,9 +1,10 @@
-"""xpu_prompt_attention where starts do not fit among many sequences."""
+"""xpu_prompt_attention at its edges: starts that do not fit among many
+sequences, out beside q in one buffer, what unseen keys hold."""
 import numpy as np
 import pytest
 
 import xpu_playground_amd as xpu
-from cache_util import GUARD, Buffers, attend, check, normal, u32, values
+from cache_util import GUARD, INF, NAN, Buffers, attend, check, normal, u32, values
 from test_gpu_prompt_attention import expected, launch
 
 pytestmark = pytest.mark.gpu
@@ -79,3 +80,21 @@ def test_out_beside_q_in_one_buffer(rt, dtype, before):
     check(values(y[:, at_out:at_out + heads * d].reshape(q.shape), dtype), want, tol)
     y[:, at_out:at_out + heads * d] = GUARD
     assert np.array_equal(y, x)
+
+
+@pytest.mark.parametrize("dtype", [xpu.BF16, xpu.FP16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("bad", ["nan", "inf"])
+@pytest.mark.parametrize("at", [1, 5, 40, 63, 64, 131, 199])
+def test_unseen_keys_change_no_bit(rt, dtype, d, bad, at):
+    """Every query before a key gives the same bits whatever the key and its
+    value are: also the queries of the tile that the key is in, whose scores of
+    it are masked and whose part of its value is 0."""
+    n, code = 200, (NAN if bad == "nan" else INF)[dtype]
+    q, k, v = normal((n, 2, d), 1, dtype), normal((n, 2, d), 2, dtype), normal((n, 2, d), 3, dtype)
+    starts = u32([0, n])
+    clean = launch(rt, q, k, v, starts, starts, dtype, shared=True)
+    k[at], v[at] = code, code
+    got = launch(rt, q, k, v, starts, starts, dtype, shared=True)
+    assert at and np.array_equal(got[:at], clean[:at])
+    assert not np.isfinite(values(got[at:], dtype)).any()

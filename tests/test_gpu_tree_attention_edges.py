@@ -1,10 +1,10 @@
-"""xpu_tree_attention where two rare things meet: rows that see nothing in
-sequences whose pages do not exist."""
+"""xpu_tree_attention at its edges: rows that see nothing of missing pages, out
+beside q in one buffer, what unseen nodes hold."""
 import numpy as np
 import pytest
 
 import xpu_playground_amd as xpu
-from cache_util import GUARD, Buffers, attend, check, normal, u32, values
+from cache_util import GUARD, INF, NAN, Buffers, attend, check, normal, u32, values
 from test_gpu_tree_attention import Case
 
 pytestmark = pytest.mark.gpu
@@ -68,3 +68,20 @@ def test_out_beside_q_in_one_buffer(rt, dtype, d, before):
     check(values(y[:, at_out:at_out + width].reshape(case.out.shape), dtype), want, tol)
     y[:, at_out:at_out + width] = GUARD
     assert np.array_equal(y, x)
+
+
+@pytest.mark.parametrize("dtype", [xpu.BF16, xpu.FP16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("bad", ["nan", "inf"])
+@pytest.mark.parametrize("context", [0, 10, 64, 3000])
+def test_unseen_nodes_change_no_bit(rt, dtype, d, bad, context):
+    """The rows that do not see a node give the same bits whatever its key and value are."""
+    case, node = Case([40, 12], [context, 50], 4, 2, d, 16, dtype, 8), 17
+    clean = case.run(rt)[0]
+    page, slot = case.tables[0, (context + node) // 16], (context + node) % 16
+    case.k[1, page, :, slot] = case.v[1, page, :, slot] = (NAN if bad == "nan" else INF)[dtype]
+    got = case.run(rt)[0]
+    blind = np.array([not m >> node & 1 for m in case.masks[0]] + [True] * (case.rows - 40), bool)
+    assert 20 < blind.sum() < case.rows
+    assert np.array_equal(got[blind], clean[blind])
+    assert not np.isfinite(values(got[~blind], dtype)).any()
