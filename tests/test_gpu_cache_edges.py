@@ -103,3 +103,35 @@ def test_append_finds_rows_among_thousands_of_sequences(rt):
                 slot = contexts[s] + i - int(starts[s])
                 pool.k[0, order[s], :, slot], pool.v[0, order[s], :, slot] = k[i], v[i]
         pool.verify()
+
+
+@pytest.mark.parametrize("starts,rows,counts", [
+    ([0, 3, 99, 5, 5, 8], 8, [2, 0, 0, 0, 1]), ([4, 2, 6, 6], 6, [0, 3, 0]), ([4, 2, 6, 6], 6, [1, 3, 1]),
+    ([0, 0xFFFFFFFF, 0, 2], 2, [0, 0, 2])])
+def test_keep_of_sequences_whose_starts_do_not_fit(rt, starts, rows, counts):
+    """They have no rows: a count of 0 gives their context as that of a sequence
+    whose starts are equal, any other is one that does not fit."""
+    n = len(counts)
+    with Buffers(rt) as b:
+        pool = Pool(rt, b, n, 2, 64, 16, 2)
+        contexts = [3 + s for s in range(n)]
+        batch = xpu.Batch(n, rows, 1, b.up(u32([[s] for s in range(n)])), b.up(u32(starts)), b.up(u32(contexts)))
+        kept = np.zeros(rows, np.uint32)
+        want, status = [], 0
+        for s, (lo, hi, count) in enumerate(zip(starts, starts[1:], counts)):
+            held = hi - lo if lo <= hi <= rows else 0
+            if count > held:
+                want.append(GUARD)
+                status = 1
+                continue
+            want.append(contexts[s] + count)
+            kept[lo:lo + count] = range(held - count, held)
+            for pools in (pool.k, pool.v):
+                old = pools.copy()
+                for j in range(count):
+                    pools[:, s, :, contexts[s] + j] = old[:, s, :, contexts[s] + held - count + j]
+        new = b.up(u32([GUARD] * n))
+        print(f"keep starts {starts} counts {counts}", flush=True)
+        rt.cache_keep(pool.cache, batch, b.up(kept), b.up(u32(counts)), new)
+        pool.verify(status=status)
+        assert list(rt.download(new, n, np.uint32)) == want

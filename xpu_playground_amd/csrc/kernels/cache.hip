@@ -88,7 +88,7 @@ template <int D> XPU_DEVICE void keep(const KeepArgs &a) {
   const uint32_t hi = __builtin_amdgcn_readfirstlane(a.batch.starts[seq + 1]);
   const uint32_t context = __builtin_amdgcn_readfirstlane(a.batch.context[seq]);
   const uint32_t count = __builtin_amdgcn_readfirstlane(a.counts[seq]);
-  if (!(lo <= hi && hi <= a.batch.rows && count <= hi - lo && count <= 64u)) {
+  if (count > (lo <= hi && hi <= a.batch.rows ? min(hi - lo, 64u) : 0u)) {
     report(a.pool);
     return;
   }
