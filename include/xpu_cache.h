@@ -90,9 +90,10 @@ int xpu_cache_append(xpu_runtime *rt, const xpu_cache *cache, const xpu_batch *b
  * out_stride elements apart; out must not overlap q (columns of one buffer, of
  * one stride, do not). FP32 scores, softmax and
  * sums; the probabilities are rounded to the cache's type for the product
- * with V. scale > 0. A page id past n_pages, a context past the table or more
- * than 64 nodes under `visible` makes the rows of that sequence NaN and sets
- * status. workspace: at least the size that xpu_tree_attention_workspace
+ * with V. (The sums are of up to 2^8 times the values, so bf16 values above 2^119
+ * / (keys) may become infinite.) scale > 0. A page id past n_pages, a context past
+ * the table or 2^31 - 1 positions, or more than 64 nodes under `visible` makes the
+ * rows of that sequence NaN and sets status. workspace: at least the size that xpu_tree_attention_workspace
  * gives for the same shapes, used from the call to its end on the stream;
  * calls on one stream may share it, graphs captured from it too. */
 int xpu_tree_attention(xpu_runtime *rt, const xpu_cache *cache, const xpu_batch *batch, uint32_t layer,

@@ -196,7 +196,9 @@ TreePlan tree_plan(const xpu_runtime &rt, const xpu_cache &c, const xpu_batch &b
   const uint64_t row_tiles = rows / (32 * p.sub_tiles) + b.n_seqs;  // at most
   const uint64_t tiles = (static_cast<uint64_t>(b.table_pitch) * c.page_size + 31) / 32;
   const bool cut = tiles > p.least;
-  // A compute unit holds two blocks. Cut into just as many as the chip holds,
+  // A compute unit holds two blocks at D 128, where all of this was measured (at
+  // D 64 four of one sub-tile or three of two; the rule is the same there, untimed).
+  // Cut into just as many as the chip holds,
   // all run at once and end together, and none starts with nothing to do (four
   // long drafts 375 us, with 3 blocks per unit dealt as others end 420; 16
   // ragged ones of 1 .. 26 nodes 36.4 and 47.0; one token behind 32000

@@ -4,10 +4,10 @@
 // one chunk, so the types and head sizes are only sizes here. Bound by memory
 // where they are large and by the launch and a chain of dependent loads (the
 // batch's numbers, the table, the rows) where they are small. Measured with 8
-// kv heads of 128: append of 48 rows 4.0 us, of the 8769 rows of 24 prompts
-// 12.8 us or 5.6 TB/s; keep of one draft in 28 layers 6.9 us, of 48 drafts
-// 11.2 us or 2.3 TB/s; copy of 4 pages of 16 6.0 us, of 101 pages of 64 in 28
-// layers 293 us or 5.1 TB/s (a large copy reaches 4.8).
+// kv heads of 128: append of 48 rows 4.1 us, of the 8769 rows of 24 prompts
+// 12.6 to 12.9 us or 5.6 TB/s; keep of one draft in 28 layers 6.9 us, of 48 drafts
+// 11.2 to 11.4 us or 2.3 TB/s; copy of 4 pages of 16 6.0 us, of 101 pages of 64 in 28
+// layers 273 to 293 us or 5.1 to 5.4 TB/s (a large copy reaches 4.8).
 #include "cache_types.hpp"
 #include "device_common.hpp"
 

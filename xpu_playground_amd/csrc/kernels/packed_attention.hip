@@ -8,17 +8,21 @@
 // so that a sequence is cut into tiles of 128 / P queries: little is lost at
 // the ends of short sequences and at the diagonal. Key tiles of 64 are staged
 // by LDS-DMA, two stages of K then V, shared by the wavefronts; two blocks to
-// a compute unit (217 registers), so one's start and end fall into the other's
-// tiles. Work is dealt heaviest first, since a last heavy tile would run alone.
+// a compute unit (220 registers; at D 64 158 and three), so one's start and end
+// fall into the other's tiles. Up to 64 sequences are dealt by the place of the
+// tile in its queries, the last places first, since a last heavy tile would run
+// alone: that is heaviest first where the sequences have equally many keys before
+// their queries, and not otherwise (a short part behind many keys comes last).
 //
-// Measured: 8192 rows, 32 heads on 8, D 128, 499 us or 1.10 PFLOP/s of the
-// causal half, 91% of what a large matrix product reaches here (the shader
-// clock, power-managed, is at 1.8 GHz with the MFMA busy in 65% of the cycles).
-// 24 sequences of 17 .. 1500 rows, the same heads, 93 us or 0.69 PFLOP/s: a
-// block has 8 tiles on average, and its queries' and result's way to memory
-// (14 us of the 93 without them) and its last, masked tile are not hidden.
-// 128 rows of 16 heads 7 us: one launch and a chain of loads. At D 64 the
-// powers bound it, 32 per lane for 16 MFMAs.
+// Measured: 8192 rows, 32 heads on 8, D 128, 468 to 514 us from box to box, 1.07
+// to 1.17 PFLOP/s of the causal half, about 90% of what a large matrix product
+// reaches here (the shader clock, power-managed, is at 1.8 GHz with the MFMA
+// busy in 64% of the cycles). 24 sequences of 17 .. 1500 rows, the same heads, 86
+// to 99 us or 0.65 to 0.75 PFLOP/s: a block has 8 tiles on average, and its
+// queries' and result's way to memory (14 us of 93 without them) and its last,
+// masked tile are not hidden. 128 rows of 16 heads 7.1 us: one launch and a chain
+// of loads. The keys are not cut, so few queries behind many keys leave most of
+// the chip idle. D 64 has as many powers for half of the MFMAs; not measured.
 #include "attention_core.hpp"
 #include "cache_types.hpp"
 
@@ -43,7 +47,8 @@ XPU_DEVICE void rows_of(const PackedArgs &a, uint32_t i, Work &w) {
 
 // Work item `rank` of up to 64 sequences, a lane each: the query tiles (1 <<
 // shift queries) of all sequences by their place in the sequence, the last
-// places first, since a tile's keys are those before it. With f(j) tiles at
+// places first, since a tile's keys are those before it (and those before the
+// sequence's queries, which are not counted here). With f(j) tiles at
 // place j or behind it, the item's place is the last j with f(j) > rank, and
 // its sequence the (rank - f(j + 1))-th that has a tile there.
 XPU_DEVICE Work heaviest_first(const PackedArgs &a, uint32_t shift, uint32_t rank) {

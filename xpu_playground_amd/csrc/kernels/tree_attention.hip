@@ -18,12 +18,15 @@
 // The cut is worked out in the kernel from starts and context (find), so a
 // call needs no lengths on the host and can be captured.
 //
+// Without masks too every row tile walks all keys of its sequence, those behind
+// its last node masked.
+//
 // Bound by the keys' way from memory: a variant without any of the arithmetic
-// takes as long. Measured with D 128 and 8 kv heads: 48 single tokens behind
+// takes as long. Measured with D 128 and 8 kv heads (D 64 has not been timed): 48 single tokens behind
 // up to 8000 positions 70 us, 5.65 TB/s; 48 drafts of 1 .. 26 nodes x 4 heads
 // the same way 89 us, 5.0 TB/s (the counters say that no key is read twice);
 // four drafts of 40 .. 64 nodes x 2 heads behind 90000 .. 131000 positions
-// 378 us, 5.0 TB/s, each key read by two blocks of 64 rows and 25% of them
+// 375 to 396 us, 4.7 to 5.0 TB/s, each key read by two blocks of 64 rows and 25% of them
 // twice from memory; of 16 nodes there, one block a key, 295 us, 6.25 TB/s;
 // one token behind 2100 positions 11.5 us, two launches and their chains of
 // loads, behind 32000 28.1 us, 4.6 TB/s. 128 rows to a
