@@ -77,6 +77,36 @@ typedef struct {
 int xpu_cache_append(xpu_runtime *rt, const xpu_cache *cache, const xpu_batch *batch, uint32_t layer,
                      const void *k, uint64_t k_stride, const void *v, uint64_t v_stride);
 
+/* How new rows are turned on their way into a cache. Per head of Q and K,
+ * in FP32 and rounded once:
+ *   n = x * gain / sqrt(mean(x^2) + eps)         where there is a gain
+ *   y_i = n_i cos - n_j sin,  y_j = n_j cos + n_i sin
+ * for the dims / 2 pairs (i, j) of the first `dims` dims, pair by pair with the
+ * entries of the row's position in the tables; the other dims stay n. */
+#define XPU_ROTARY_HALVES 0   /* pair p: dims p and p + dims / 2 */
+#define XPU_ROTARY_ADJACENT 1 /* pair p: dims 2 p and 2 p + 1 */
+typedef struct {
+  uint32_t positions;       /* rows of the tables */
+  uint32_t dims;            /* a multiple of 16, at most head_dim */
+  int32_t pairs;            /* XPU_ROTARY_HALVES or XPU_ROTARY_ADJACENT */
+  float eps;                /* >= 0 */
+  const float *cos, *sin;   /* device, [positions][dims / 2], 16-byte aligned */
+  const uint32_t *at;       /* device, the position of each row of the batch (nodes of
+                               a tree share depths); NULL: its position in the cache */
+  const void *q_gain, *k_gain; /* device, [head_dim] of the cache's type, or NULL */
+} xpu_rotary;
+
+/* xpu_cache_append with Q and K normalised and rotated on the way. V is stored
+ * as it is. heads > 0: Q ([rows][heads][head_dim], q_stride apart) is turned
+ * too and goes to q_out, which may be q itself with its stride and otherwise
+ * overlaps no input; heads 0: q and q_out are not looked at. A row whose
+ * position is not in the tables is not written, its q_out is NaN, and sets
+ * status; its q_out is written also where its place in the cache does not
+ * exist. */
+int xpu_cache_append_rotary(xpu_runtime *rt, const xpu_cache *cache, const xpu_batch *batch, uint32_t layer,
+                            const xpu_rotary *rotary, uint32_t heads, const void *q, uint64_t q_stride, void *q_out,
+                            uint64_t out_stride, const void *k, uint64_t k_stride, const void *v, uint64_t v_stride);
+
 /* Attention of the batch's rows, which are in the cache already (appended):
  * a row sees all context[s] positions before the batch's and, of the
  * sequence's own rows ("nodes"), node j when bit j of visible[row] is set

@@ -1,7 +1,8 @@
 """ctypes bindings to the gfx950 hot-path library (build/libxpu_playground.so).
 
 The C ABI is declared in include/xpu_runtime.h, include/xpu_kernels.h,
-include/xpu_qwen3.h and include/xpu_cache.h. Every compute call runs the HIP kernels of
+include/xpu_qwen3.h, include/xpu_cache.h, include/xpu_cache8.h and
+include/xpu_sample.h. Every compute call runs the HIP kernels of
 build/xpu_kernels.hsaco; there is no CPU fallback: if the library or the code
 object is missing, or no gfx950 device is visible, the calls raise.
 """
@@ -21,6 +22,12 @@ MODULE_PATH = os.path.join(BUILD_DIR, "xpu_kernels.hsaco")
 
 BF16 = 0
 FP16 = 1
+FP32 = 2  # of logits (Sampling)
+
+HALVES = 0  # pairs of a rotation (Rotary)
+ADJACENT = 1
+
+SAMPLE_NONE = 0xFFFFFFFF  # the token of a row without an answer (Runtime.sample)
 
 XPU_OK = 0
 
@@ -109,6 +116,72 @@ class Cache(ctypes.Structure):
                  n_pages * page if layer_stride is None else layer_stride, page if page_stride is None else page_stride)
         _fit("Cache", self._sizes, *sizes)
         super().__init__(*sizes, k, v, status)
+
+
+class Cache8(ctypes.Structure):
+    """xpu_cache8 (include/xpu_cache8.h): the pages of a KV cache in 8 bits. k
+    and v are device addresses, strides are in bytes; without strides the pools
+    are [layers][n_pages][page_bytes], page_bytes being a page's codes and
+    scales, rounded up to 128."""
+
+    _fields_ = Cache._fields_
+    _sizes = Cache._sizes
+
+    def __init__(self, dtype, layers, kv_heads, head_dim, page_size, n_pages, k=None, v=None, status=None,
+                 layer_stride=None, page_stride=None):
+        if page_stride is None:
+            page_stride = -(-(kv_heads * page_size * head_dim + kv_heads * (page_size // 16)) // 128) * 128
+        sizes = (dtype, layers, kv_heads, head_dim, page_size, n_pages,
+                 n_pages * page_stride if layer_stride is None else layer_stride, page_stride)
+        _fit("Cache8", self._sizes, *sizes)
+        super().__init__(*sizes, k, v, status)
+
+
+class Rotary(ctypes.Structure):
+    """xpu_rotary (include/xpu_cache.h): how new Q and K rows are turned. cos
+    and sin are device addresses of FP32 [positions][dims / 2], at of uint32
+    per row, the gains of head_dim elements of the cache's type."""
+
+    _fields_ = [
+        ("positions", c_uint32),
+        ("dims", c_uint32),
+        ("pairs", c_int),
+        ("eps", c_float),
+        ("cos", c_void_p),
+        ("sin", c_void_p),
+        ("at", c_void_p),
+        ("q_gain", c_void_p),
+        ("k_gain", c_void_p),
+    ]
+    _sizes = struct.Struct("2Ii")
+
+    def __init__(self, positions, dims, cos=None, sin=None, pairs=HALVES, at=None, q_gain=None, k_gain=None, eps=1e-6):
+        _fit("Rotary", self._sizes, positions, dims, pairs)
+        super().__init__(positions, dims, pairs, eps, cos, sin, at, q_gain, k_gain)
+
+
+class Sampling(ctypes.Structure):
+    """xpu_sampling (include/xpu_sample.h): how the rows' tokens are drawn.
+    random, temperature, top_k, top_p and min_p are device addresses, a number
+    per row; without a stride the rows are dense."""
+
+    _fields_ = [
+        ("dtype", c_int),
+        ("rows", c_uint32),
+        ("vocab", c_uint32),
+        ("stride", c_uint64),
+        ("temperature", c_void_p),
+        ("top_k", c_void_p),
+        ("top_p", c_void_p),
+        ("min_p", c_void_p),
+        ("random", c_void_p),
+    ]
+    _sizes = struct.Struct("i2IQ")
+
+    def __init__(self, dtype, rows, vocab, random=None, temperature=None, top_k=None, top_p=None, min_p=None, stride=None):
+        sizes = (dtype, rows, vocab, vocab if stride is None else stride)
+        _fit("Sampling", self._sizes, *sizes)
+        super().__init__(*sizes, temperature, top_k, top_p, min_p, random)
 
 
 class Batch(ctypes.Structure):
@@ -280,6 +353,31 @@ def _declare(lib):
         ),
         "xpu_cache_keep": (c_int, [c_void_p, POINTER(Cache), POINTER(Batch), c_void_p, c_void_p, c_void_p]),
         "xpu_cache_copy": (c_int, [c_void_p, POINTER(Cache), c_void_p, c_void_p, c_uint32]),
+        "xpu_cache_append_rotary": (
+            c_int,
+            [c_void_p, POINTER(Cache), POINTER(Batch), c_uint32, POINTER(Rotary), c_uint32] + [c_void_p, c_uint64] * 4,
+        ),
+        "xpu_cache8_page_bytes": (c_int, [POINTER(Cache8), POINTER(c_uint64)]),
+        "xpu_cache8_append": (
+            c_int,
+            [c_void_p, POINTER(Cache8), POINTER(Batch), c_uint32, POINTER(Rotary), c_uint32] + [c_void_p, c_uint64] * 4,
+        ),
+        "xpu_tree_attention8": (
+            c_int,
+            [c_void_p, POINTER(Cache8), POINTER(Batch), c_uint32, c_uint32, c_float, c_void_p, c_uint64, c_void_p]
+            + [c_void_p, c_uint64] * 2,
+        ),
+        "xpu_tree_attention8_workspace": (
+            c_int,
+            [c_void_p, POINTER(Cache8), POINTER(Batch), c_uint32, POINTER(c_uint64)],
+        ),
+        "xpu_cache8_keep": (c_int, [c_void_p, POINTER(Cache8), POINTER(Batch), c_void_p, c_void_p, c_void_p]),
+        "xpu_cache8_copy": (c_int, [c_void_p, POINTER(Cache8), c_void_p, c_void_p, c_uint32]),
+        "xpu_sample": (
+            c_int,
+            [c_void_p, POINTER(Sampling), c_void_p, c_void_p, c_void_p, c_void_p, c_uint64],
+        ),
+        "xpu_sample_workspace": (c_int, [c_void_p, POINTER(Sampling), POINTER(c_uint64)]),
         "xpu_prompt_attention": (c_int, [c_void_p, POINTER(Packed), c_void_p, c_void_p, c_void_p, c_void_p]),
         "xpu_pages_create": (c_int, [c_uint32, POINTER(c_void_p)]),
         "xpu_pages_destroy": (None, [c_void_p]),
@@ -530,6 +628,70 @@ class Runtime:
         if len(s) != len(d):
             raise ValueError("src and dst must be of one length")
         check(self.lib.xpu_cache_copy(self.handle, cache, s.ctypes.data, d.ctypes.data, len(s)))
+
+    def cache_append_rotary(self, cache: Cache, batch: Batch, layer: int, k: int, v: int, rotary: Rotary,
+                            heads: int = 0, q: int | None = None, q_out: int | None = None,
+                            k_stride: int | None = None, v_stride: int | None = None, q_stride: int | None = None,
+                            out_stride: int | None = None) -> None:
+        """cache_append with K, and with `heads` Q on its way to q_out, turned."""
+        self._append_turned(self.lib.xpu_cache_append_rotary, cache, batch, layer, k, v, rotary, heads, q, q_out,
+                            k_stride, v_stride, q_stride, out_stride)
+
+    def _append_turned(self, call, cache, batch, layer, k, v, rotary, heads, q, q_out, k_stride, v_stride, q_stride,
+                       out_stride):
+        dense, q_dense = cache.kv_heads * cache.head_dim, heads * cache.head_dim
+        check(call(self.handle, cache, batch, layer, rotary, heads, q, q_dense if q_stride is None else q_stride, q_out,
+                   q_dense if out_stride is None else out_stride, k, dense if k_stride is None else k_stride, v,
+                   dense if v_stride is None else v_stride))
+
+    def cache8_page_bytes(self, cache: Cache8) -> int:
+        """Bytes of a page, codes and scales."""
+        v = c_uint64()
+        check(self.lib.xpu_cache8_page_bytes(cache, ctypes.byref(v)))
+        return v.value
+
+    def cache8_append(self, cache: Cache8, batch: Batch, layer: int, k: int, v: int, rotary: Rotary | None = None,
+                      heads: int = 0, q: int | None = None, q_out: int | None = None, k_stride: int | None = None,
+                      v_stride: int | None = None, q_stride: int | None = None, out_stride: int | None = None) -> None:
+        self._append_turned(self.lib.xpu_cache8_append, cache, batch, layer, k, v, rotary, heads, q, q_out, k_stride,
+                            v_stride, q_stride, out_stride)
+
+    def tree_attention8_workspace(self, cache: Cache8, batch: Batch, heads: int) -> int:
+        """Bytes of workspace that tree_attention8 needs for these shapes."""
+        v = c_uint64()
+        check(self.lib.xpu_tree_attention8_workspace(self.handle, cache, batch, heads, ctypes.byref(v)))
+        return v.value
+
+    def tree_attention8(self, cache: Cache8, batch: Batch, layer: int, heads: int, q: int, out: int,
+                        workspace: int | None, workspace_bytes: int, visible: int | None = None,
+                        scale: float | None = None, q_stride: int | None = None, out_stride: int | None = None) -> None:
+        dense = heads * cache.head_dim
+        check(self.lib.xpu_tree_attention8(self.handle, cache, batch, layer, heads,
+                                           cache.head_dim ** -0.5 if scale is None else scale, q,
+                                           dense if q_stride is None else q_stride, visible, out,
+                                           dense if out_stride is None else out_stride, workspace, workspace_bytes))
+
+    def cache8_keep(self, cache: Cache8, batch: Batch, kept: int, counts: int, new_context: int | None = None) -> None:
+        check(self.lib.xpu_cache8_keep(self.handle, cache, batch, kept, counts, new_context))
+
+    def cache8_copy(self, cache: Cache8, src, dst) -> None:
+        """src, dst: page ids on the host (arrays or lists of one length)."""
+        s, d = page_ids(src), page_ids(dst)
+        if len(s) != len(d):
+            raise ValueError("src and dst must be of one length")
+        check(self.lib.xpu_cache8_copy(self.handle, cache, s.ctypes.data, d.ctypes.data, len(s)))
+
+    # ---- tokens from logits (include/xpu_sample.h)
+    def sample_workspace(self, sampling: Sampling) -> int:
+        """Bytes of workspace that sample needs for these shapes."""
+        v = c_uint64()
+        check(self.lib.xpu_sample_workspace(self.handle, sampling, ctypes.byref(v)))
+        return v.value
+
+    def sample(self, sampling: Sampling, logits: int, tokens: int, workspace: int | None = None,
+               workspace_bytes: int = 0, probability: int | None = None) -> None:
+        """A token of every row (uint32), and its share of the kept weight (FP32)."""
+        check(self.lib.xpu_sample(self.handle, sampling, logits, tokens, probability, workspace, workspace_bytes))
 
     def prompt_attention(self, packed: Packed, q: int, k: int, v: int, out: int) -> None:
         check(self.lib.xpu_prompt_attention(self.handle, packed, q, k, v, out))

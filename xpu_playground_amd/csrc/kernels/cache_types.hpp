@@ -93,6 +93,42 @@ struct KeepArgs {
   uint32_t *new_context;
 };
 
+// The rotation of rows on their way (half = rotated dims / 2; 0: none).
+struct RotaryArgs {
+  const float *cos, *sin;  // [positions][half]
+  const uint32_t *at;
+  const uint16_t *q_gain, *k_gain;
+  uint32_t positions, half, adjacent;
+  float eps;
+};
+
+// New rows, Q with them where heads > 0. Of an 8-bit cache, pool.k and pool.v
+// are the codes, and strides of the pool are in bytes.
+struct RotateArgs {
+  PoolArgs pool;
+  BatchArgs batch;
+  RotaryArgs rot;
+  const uint16_t *q, *k, *v;
+  uint16_t *q_out;
+  uint64_t q_stride, k_stride, v_stride, out_stride;  // elements
+  uint32_t heads;
+  uint32_t parts;  // wavefronts that share a row
+  uint32_t slots;  // 8 bits: blocks of positions that the batch reaches, at most
+};
+
+// An 8-bit cache's positions share scales by blocks of 16: 2^(byte - 127).
+constexpr uint32_t kBlock = 16, kLeastScale = 27, kMostScale = 247;
+
+// A sequence's blocks that rows lo .. hi - 1 behind c positions reach.
+XPU_BOTH uint32_t blocks_of(uint32_t n, uint32_t c) { return n ? ((c & (kBlock - 1u)) + n + kBlock - 1u) / kBlock : 0u; }
+
+// The scale byte with which a float of these bits (a finite one, without its
+// sign) is at most 448, the largest code: 1.75 * 2^8.
+XPU_BOTH uint32_t scale_for(uint32_t bits) {
+  const uint32_t e = bits >> 23, s = (bits & 0x7fffffu) > 0x600000u ? e + 1u : e;
+  return s < kLeastScale + 8u ? kLeastScale : s - 8u;
+}
+
 constexpr uint32_t kCopyPairs = 400;  // per launch; the arguments stay below 4 KiB
 struct CopyArgs {
   PoolArgs pool;

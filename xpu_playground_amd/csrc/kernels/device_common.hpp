@@ -201,6 +201,7 @@ XPU_DEVICE u32x4 load_nt16(const void *p) {
 // ------------------------------------------------ global -> LDS DMA (gfx950)
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
 
 // Raw buffer descriptor: 48-bit base, stride 0, num_records bytes, 32-bit
 // data format. Offsets at or past num_records read as zero.

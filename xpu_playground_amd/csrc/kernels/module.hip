@@ -17,5 +17,9 @@ __device__ uint32_t xpu_stamp_phase[xpu::kPhaseSlots * xpu::kStampRing * xpu::kP
 #include "prefill_attention.hip"
 #include "packed_attention.hip"
 #include "tree_attention.hip"
+#include "tree_attention8.hip"
 #include "cache.hip"
+#include "rotary.hip"
+#include "cache8.hip"
+#include "sample.hip"
 #include "peak.hip"

@@ -135,6 +135,72 @@ template <int R, typename Is> XPU_DEVICE Place find(const TreeArgs &a, uint32_t 
 // (max, sum) pairs.
 template <int D, int R> constexpr uint32_t kPartial = 32u * R * (D + 2u);
 
+// The wavefronts' results meet in LDS, a sub-tile at a time; each wavefront
+// adds up a quarter of the columns (kMine registers of every lane's D / 2),
+// in the order of the keys. A side without a finite score has only zeros or
+// NaN in its sum, which stay. `bad` makes the rows NaN.
+// po: D / 2 columns of 64 floats per wavefront, meet: 128 floats per wavefront.
+template <int DT, int D, int R>
+XPU_DEVICE void finish(const TreeArgs &a, const Rows<DT, D, R> &rows, const Place &place, const uint64_t (&sees)[R],
+                       uint32_t item, bool bad, float *po, float *meet) {
+  const uint32_t lane = lane_id(), hh = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t kvh = blockIdx.x % a.pool.kv_heads, group = a.heads / a.pool.kv_heads;
+  const Sequence &s = place.s;
+  const uint32_t row_tile = (item - place.first) % s.row_tiles, rows_in = min(s.n * group - row_tile * 32u * R, 32u * R);
+  constexpr uint32_t kMine = D / 8;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    __syncthreads();  // the tiles, the queries, the sub-tile before are read
+    meet[(wave * 2u) * 64u + lane] = rows.m[r];
+    meet[(wave * 2u + 1u) * 64u + lane] = bad ? __builtin_nanf("") : rows.total(r);
+#pragma unroll
+    for (uint32_t dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (uint32_t i = 0; i < 16; ++i) po[(wave * (D / 2u) + dt * 16u + i) * 64u + lane] = rows.o[r][dt][i];
+    __syncthreads();
+    const float ninf = -__builtin_inff();
+    float m[4], x[4], top = ninf, sum = 0.0f;
+#pragma unroll
+    for (uint32_t w = 0; w < 4; ++w) top = fmaxf(top, m[w] = meet[w * 128u + lane]);
+#pragma unroll
+    for (uint32_t w = 0; w < 4; ++w) {
+      const float side = meet[w * 128u + 64u + lane];
+      x[w] = m[w] == ninf ? 0.0f : __builtin_amdgcn_exp2f((m[w] - top) * a.scale_log2e);
+      sum += m[w] == ninf ? side : side * x[w];
+    }
+    float o[kMine];
+#pragma unroll
+    for (uint32_t i = 0; i < kMine; ++i) {
+      o[i] = 0.0f;
+#pragma unroll
+      for (uint32_t w = 0; w < 4; ++w)
+        o[i] = __builtin_fmaf(po[(w * (D / 2u) + wave * kMine + i) * 64u + lane], x[w], o[i]);
+    }
+    // register wave * kMine + i: dims 32 (reg / 16) + 8 (reg % 16 / 4) + 4 hh + reg % 4
+    const uint32_t in = 32u * r + (lane & 31u), row = row_tile * 32u * R + in;
+    const uint32_t dim = wave * 2u * kMine + 4u * hh;
+    if (in >= rows_in) continue;
+    if (place.chunks == 1) {
+      // (the sum has the NaN of every wavefront that met a missing page)
+      const bool empty = s.context == 0 && a.visible && sees[r] == 0 && sum == 0.0f;
+      const float by = empty ? 0.0f : 1.0f / sum;
+      uint16_t *to = a.out + (s.first + row / group) * a.out_stride + (kvh * group + row % group) * D + dim;
+#pragma unroll
+      for (uint32_t w = 0; w < kMine / 4; ++w)
+        *reinterpret_cast<u32x2 *>(to + 8u * w) = u32x2{dma::cvt_pack<DT>(o[4 * w] * by, o[4 * w + 1] * by),
+                                                        dma::cvt_pack<DT>(o[4 * w + 2] * by, o[4 * w + 3] * by)};
+    } else {
+      float *slot = a.partial + (static_cast<uint64_t>(item) * a.pool.kv_heads + kvh) * kPartial<D, R>;
+      float *to = slot + in * D + dim;
+#pragma unroll
+      for (uint32_t w = 0; w < kMine / 4; ++w)
+        *reinterpret_cast<dma::f32x4 *>(to + 8u * w) = dma::f32x4{o[4 * w], o[4 * w + 1], o[4 * w + 2], o[4 * w + 3]};
+      if (wave == 0 && hh == 0)
+        *reinterpret_cast<dma::f32x2 *>(slot + 32u * R * D + 2u * in) = dma::f32x2{top, sum};
+    }
+  }
+}
+
 template <int DT, int D, int R> XPU_DEVICE void tree_attention(const TreeArgs &a) {
   constexpr uint32_t kRow = 2u * D, kTile = kTreeKeys * kRow;
   constexpr uint32_t kRpi = 512u / D, kCpr = D / 8;
@@ -157,7 +223,6 @@ template <int DT, int D, int R> XPU_DEVICE void tree_attention(const TreeArgs &a
   const uint32_t seq = static_cast<uint32_t>(place.seq);
   const Sequence &s = place.s;
   const uint32_t row_tile = (item - place.first) % s.row_tiles, chunk = (item - place.first) / s.row_tiles;
-  const uint32_t rows_in = min(s.n * group - row_tile * 32u * R, 32u * R);
   // the chunk's tiles, and the wave's share of them
   const uint32_t c0 = static_cast<uint32_t>(static_cast<uint64_t>(s.tiles) * chunk / place.chunks);
   const uint32_t c1 = static_cast<uint32_t>(static_cast<uint64_t>(s.tiles) * (chunk + 1u) / place.chunks);
@@ -317,64 +382,8 @@ template <int DT, int D, int R> XPU_DEVICE void tree_attention(const TreeArgs &a
     if (more) issue(a.pool.v, lds0 + kTile, v_off);
   }
 
-  // The wavefronts' results meet in LDS, a sub-tile at a time; each wavefront
-  // adds up a quarter of the columns (kMine registers of every lane's D / 2),
-  // in the order of the keys. A side without a finite score has only zeros or
-  // NaN in its sum, which stay. `bad` makes the rows NaN.
   if (bad && lane == 0 && a.pool.status) *a.pool.status = 1u;
-  constexpr uint32_t kMine = D / 8;
-  float *po = reinterpret_cast<float *>(lds), *meet = reinterpret_cast<float *>(shared_q);
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    __syncthreads();  // the tiles, the queries, the sub-tile before are read
-    meet[(wave * 2u) * 64u + lane] = rows.m[r];
-    meet[(wave * 2u + 1u) * 64u + lane] = bad ? __builtin_nanf("") : rows.total(r);
-#pragma unroll
-    for (uint32_t dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-      for (uint32_t i = 0; i < 16; ++i) po[(wave * (D / 2u) + dt * 16u + i) * 64u + lane] = rows.o[r][dt][i];
-    __syncthreads();
-    const float ninf = -__builtin_inff();
-    float m[4], x[4], top = ninf, sum = 0.0f;
-#pragma unroll
-    for (uint32_t w = 0; w < 4; ++w) top = fmaxf(top, m[w] = meet[w * 128u + lane]);
-#pragma unroll
-    for (uint32_t w = 0; w < 4; ++w) {
-      const float side = meet[w * 128u + 64u + lane];
-      x[w] = m[w] == ninf ? 0.0f : __builtin_amdgcn_exp2f((m[w] - top) * a.scale_log2e);
-      sum += m[w] == ninf ? side : side * x[w];
-    }
-    float o[kMine];
-#pragma unroll
-    for (uint32_t i = 0; i < kMine; ++i) {
-      o[i] = 0.0f;
-#pragma unroll
-      for (uint32_t w = 0; w < 4; ++w)
-        o[i] = __builtin_fmaf(po[(w * (D / 2u) + wave * kMine + i) * 64u + lane], x[w], o[i]);
-    }
-    // register wave * kMine + i: dims 32 (reg / 16) + 8 (reg % 16 / 4) + 4 hh + reg % 4
-    const uint32_t in = 32u * r + (lane & 31u), row = row_tile * 32u * R + in;
-    const uint32_t dim = wave * 2u * kMine + 4u * hh;
-    if (in >= rows_in) continue;
-    if (place.chunks == 1) {
-      // (the sum has the NaN of every wavefront that met a missing page)
-      const bool empty = s.context == 0 && a.visible && sees[r] == 0 && sum == 0.0f;
-      const float by = empty ? 0.0f : 1.0f / sum;
-      uint16_t *to = a.out + (s.first + row / group) * a.out_stride + (kvh * group + row % group) * D + dim;
-#pragma unroll
-      for (uint32_t w = 0; w < kMine / 4; ++w)
-        *reinterpret_cast<u32x2 *>(to + 8u * w) = u32x2{dma::cvt_pack<DT>(o[4 * w] * by, o[4 * w + 1] * by),
-                                                        dma::cvt_pack<DT>(o[4 * w + 2] * by, o[4 * w + 3] * by)};
-    } else {
-      float *slot = a.partial + (static_cast<uint64_t>(item) * a.pool.kv_heads + kvh) * kPartial<D, R>;
-      float *to = slot + in * D + dim;
-#pragma unroll
-      for (uint32_t w = 0; w < kMine / 4; ++w)
-        *reinterpret_cast<dma::f32x4 *>(to + 8u * w) = dma::f32x4{o[4 * w], o[4 * w + 1], o[4 * w + 2], o[4 * w + 3]};
-      if (wave == 0 && hh == 0)
-        *reinterpret_cast<dma::f32x2 *>(slot + 32u * R * D + 2u * in) = dma::f32x2{top, sum};
-    }
-  }
+  finish<DT, D, R>(a, rows, place, sees, item, bad, reinterpret_cast<float *>(lds), reinterpret_cast<float *>(shared_q));
 }
 
 // Reductions over each half-wave: partners l ^ 16, 8, 4, 2, 1 of wave_reduce.
