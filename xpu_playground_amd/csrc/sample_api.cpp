@@ -1,5 +1,5 @@
 // Entry points of the sampling (include/xpu_sample.h): argument checks and the
-// launch. Kernel: kernels/sample.hip.
+// launches. Kernels: kernels/sample.hip.
 #include "../../include/xpu_sample.h"
 #include "cache_checks.hpp"
 #include "kernels/sample_types.hpp"
@@ -25,6 +25,31 @@ int check_sampling(const char *name, const xpu_sampling *s, bool memory) {
   return XPU_OK;
 }
 
+// How a call is cut (kernels/sample.hip), by the numbers of rows and tokens
+// alone: parts of a row, 0 for one launch.
+struct SamplePlan {
+  uint32_t parts = 0, chunk = 0;
+  uint64_t firsts = 0, lists = 0, weights = 0, numbers = 0, listed = 0, groups = 0, bytes = 0;  // offsets; in all
+};
+
+SamplePlan sample_plan(const xpu_runtime &rt, const xpu_sampling &s) {
+  SamplePlan p;
+  if (s.vocab < 16384) return p;
+  p.parts = 1;
+  while (p.parts < xpu::kSampleParts && 2ull * p.parts * s.rows <= 2ull * rt.compute_units &&
+         s.vocab / (2 * p.parts) >= 4096)
+    p.parts *= 2;
+  p.chunk = (s.vocab + 8 * p.parts - 1) / (8 * p.parts) * 8;
+  const uint64_t blocks = static_cast<uint64_t>(s.rows) * p.parts;
+  p.lists = p.firsts + 8 * blocks;
+  p.weights = p.lists + 8 * blocks * xpu::kSampleCap;
+  p.numbers = p.weights + 8 * blocks * xpu::kSampleSlots;
+  p.listed = p.numbers + 4 * blocks * xpu::kSampleSlots;
+  p.groups = p.listed + 4 * blocks;
+  p.bytes = p.groups + 4ull * s.rows * xpu::kSampleThreads;
+  return p;
+}
+
 }  // namespace
 
 extern "C" {
@@ -35,7 +60,7 @@ int xpu_sample_workspace(const xpu_runtime *rt, const xpu_sampling *sampling, ui
     if (!bytes) return invalid(name, "null output");
     if (int rc = check_sampling(name, sampling, false)) return rc;
     if (int rc = check_runtime(name, rt)) return rc;
-    *bytes = 0;
+    *bytes = sampling->rows ? sample_plan(*rt, *sampling).bytes : 0;
     return XPU_OK;
   });
 }
@@ -62,8 +87,9 @@ int xpu_sample(xpu_runtime *rt, const xpu_sampling *sampling, const void *logits
           return invalid(name, "tokens and probability must not overlap the numbers of the rows");
     }
     if (int rc = check_runtime(name, rt)) return rc;
-    (void)workspace;
-    (void)workspace_bytes;
+    const SamplePlan plan = sample_plan(*rt, s);
+    if (plan.bytes && (!workspace || !aligned(workspace, 16) || workspace_bytes < plan.bytes))
+      return invalid(name, "needs a workspace of " + std::to_string(plan.bytes) + " bytes, 16-byte aligned");
     xpu::SampleArgs a{};
     a.logits = logits;
     a.stride = s.stride;
@@ -75,10 +101,25 @@ int xpu_sample(xpu_runtime *rt, const xpu_sampling *sampling, const void *logits
     a.tokens = tokens;
     a.probability = probability;
     a.vocab = s.vocab;
-    a.bits = 62;
-    while ((1ull << (62 - a.bits)) < s.vocab) --a.bits;
-    const char *kernel = s.dtype == XPU_DTYPE_FP32 ? "xpu_sample_fp32" : s.dtype == XPU_DTYPE_FP16 ? "xpu_sample_fp16" : "xpu_sample_bf16";
-    return launch(rt, kernel, s.rows, a, 1, nullptr, 1024);
+    a.fine = 44;
+    while ((1ull << (61 - a.fine)) < s.vocab) --a.fine;
+    const std::string form =
+        s.dtype == XPU_DTYPE_FP32 ? "_fp32" : s.dtype == XPU_DTYPE_FP16 ? "_fp16" : "_bf16";
+    if (plan.parts) {
+      uint8_t *w = static_cast<uint8_t *>(workspace);
+      a.parts = plan.parts;
+      a.chunk = plan.chunk;
+      a.firsts = reinterpret_cast<uint64_t *>(w + plan.firsts);
+      a.lists = reinterpret_cast<uint64_t *>(w + plan.lists);
+      a.weights = reinterpret_cast<uint64_t *>(w + plan.weights);
+      a.numbers = reinterpret_cast<uint32_t *>(w + plan.numbers);
+      a.listed = reinterpret_cast<uint32_t *>(w + plan.listed);
+      a.groups = reinterpret_cast<float *>(w + plan.groups);
+      const uint64_t blocks = static_cast<uint64_t>(s.rows) * plan.parts;
+      if (int rc = launch(rt, "xpu_sample_look" + form, blocks, a, 1, nullptr, xpu::kSampleThreads)) return rc;
+      if (int rc = launch(rt, "xpu_sample_list" + form, blocks, a, 1, nullptr, xpu::kSampleThreads)) return rc;
+    }
+    return launch(rt, "xpu_sample_draw" + form, s.rows, a, 1, nullptr, xpu::kSampleThreads);
   });
 }
 
