@@ -31,9 +31,10 @@ extern "C" {
  * The token is the first of the order at which the weights up to it pass random
  * times the kept ones' sum. Temperature 0 keeps the first token alone. A logit
  * of -infinity is never drawn. The numbers of the rows are on the device, one
- * per row; NULL is temperature 1, or no filter. Weights and sums have 64 bits;
- * sums are exact to 2^-42 of the largest weight per token, whatever their
- * order, so a row's token does not depend on the rows beside it. */
+ * per row; NULL is temperature 1, or no filter. Weights are formed in 64 bits
+ * and summed as integers, off by half of 2^-41 of the largest weight per token
+ * at most (2^-44 up to 2^17 tokens) in any order, so a row's token does not
+ * depend on the rows beside it; a weight below 2^-47 of the largest is 0. */
 typedef struct {
   int32_t dtype;            /* of the logits: XPU_DTYPE_BF16, _FP16 or _FP32 */
   uint32_t rows;

@@ -162,6 +162,34 @@ def test_masked_tokens(rt, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [9000, 40000, 151936])
+def test_few_tokens_that_are_not_masked(rt, dtype, vocab):
+    """Whole parts of a row are -infinity or the type's lowest number, first,
+    last or in between."""
+    lowest = float(torch.finfo(TORCH[dtype]).min)
+    x = logits(8, vocab, 13)
+    for i, mask in enumerate((-np.inf, lowest)):
+        x[4 * i, : vocab - 5] = mask
+        x[4 * i + 1, 5:] = mask
+        x[4 * i + 2, : vocab // 2] = x[4 * i + 2, vocab // 2 + 3000:] = mask
+        x[4 * i + 3, np.random.RandomState(i).permutation(vocab)[: vocab - 40]] = mask
+    for k in (0, 20, 300):
+        for p in (1.0, 0.9):
+            Rows(x, dtype, t=0.8, k=k, p=p, m=0.001).verify(rt)
+            Rows(x, dtype, t=3e38, k=k, p=p).verify(rt)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_logits_that_rise_and_fall(rt, dtype):
+    """The largest so far changes all the way through a row, and by powers of
+    two beyond those that the histogram holds at a time."""
+    at = np.arange(50000)
+    x = np.stack([at * 2e-4, 10 - at * 2e-4, at * 0.01 - 500, 500 - at * 0.01, np.sin(at / 3000) * 90, at // 1000 * 20.0 - 999])
+    for numbers in (dict(), dict(p=0.95), dict(k=2000, p=0.9), dict(k=30), dict(m=0.2), dict(t=7.0, p=0.7)):
+        Rows(x, dtype, **numbers).verify(rt)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_numbers_out_of_range(rt, dtype):
     x = logits(1, 500, 7)
     bad = [dict(t=-1.0), dict(t=np.nan), dict(t=np.inf), dict(p=-0.1), dict(p=np.nan), dict(m=-0.1), dict(m=1.5),

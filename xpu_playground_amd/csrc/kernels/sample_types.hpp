@@ -6,9 +6,9 @@
 
 namespace xpu {
 
-// Places of a part's histogram, entries of its list, threads of a block, parts
-// of a row at most.
-constexpr uint32_t kSampleSlots = 2048, kSampleCap = 1024, kSampleThreads = 1024, kSampleParts = 16;
+// Places of a part's histogram, entries of its list, threads of a block of the
+// first two launches and of the last, parts of a row at most.
+constexpr uint32_t kSampleSlots = 2048, kSampleCap = 4096, kSampleThreads = 1024, kSampleDraw = 256, kSampleParts = 16;
 
 struct SampleArgs {
   const void *logits;

@@ -36,7 +36,7 @@ SamplePlan sample_plan(const xpu_runtime &rt, const xpu_sampling &s) {
   SamplePlan p;
   if (s.vocab < 16384) return p;
   p.parts = 1;
-  while (p.parts < xpu::kSampleParts && 2ull * p.parts * s.rows <= 2ull * rt.compute_units &&
+  while (p.parts < xpu::kSampleParts && 2ull * p.parts * s.rows <= rt.compute_units &&
          s.vocab / (2 * p.parts) >= 4096)
     p.parts *= 2;
   p.chunk = (s.vocab + 8 * p.parts - 1) / (8 * p.parts) * 8;
@@ -119,7 +119,7 @@ int xpu_sample(xpu_runtime *rt, const xpu_sampling *sampling, const void *logits
       if (int rc = launch(rt, "xpu_sample_look" + form, blocks, a, 1, nullptr, xpu::kSampleThreads)) return rc;
       if (int rc = launch(rt, "xpu_sample_list" + form, blocks, a, 1, nullptr, xpu::kSampleThreads)) return rc;
     }
-    return launch(rt, "xpu_sample_draw" + form, s.rows, a, 1, nullptr, xpu::kSampleThreads);
+    return launch(rt, "xpu_sample_draw" + form, s.rows, a, 1, nullptr, xpu::kSampleDraw);
   });
 }
 
