@@ -107,11 +107,12 @@ xpu::RotateArgs rotate_args(const xpu::PoolArgs &pool, const Rows &r) {
   return a;
 }
 
-// Wavefronts that share a row of `heads` heads: all that it has work for while
-// there are fewer than the chip holds.
+// Wavefronts that share a row of `heads` heads: as many as there is work for
+// while there are fewer than the chip holds, else each has what it loads at a
+// time (kernels/rotary.hip).
 uint32_t parts_of(const xpu_runtime &rt, uint32_t rows, uint32_t heads, uint32_t head_dim) {
   const uint64_t most = (heads * (head_dim / 8ull) + 63) / 64, room = rt.compute_units * 16ull / rows;
-  return static_cast<uint32_t>(std::max<uint64_t>(1, std::min(most, room)));
+  return static_cast<uint32_t>(std::max<uint64_t>((most + 3) / 4, std::min(most, room)));
 }
 
 std::string form_of(int32_t dtype, uint32_t head_dim) {
@@ -142,7 +143,7 @@ int xpu_cache_append_rotary(xpu_runtime *rt, const xpu_cache *cache, const xpu_b
     a.parts = parts_of(*rt, batch->rows, heads + 2 * cache->kv_heads, cache->head_dim);
     const uint64_t waves = static_cast<uint64_t>(batch->rows) * a.parts;
     return launch(rt, "xpu_cache_append_rotary" + form_of(cache->dtype, cache->head_dim),
-                  std::min<uint64_t>((waves + 3) / 4, rt->compute_units * 8ull), a);
+                  std::min<uint64_t>((waves + 3) / 4, rt->compute_units * 64ull), a);
   });
 }
 
@@ -179,7 +180,7 @@ int xpu_cache8_append(xpu_runtime *rt, const xpu_cache8 *cache, const xpu_batch 
     const uint64_t waves =
         2ull * cache->kv_heads * a.slots + static_cast<uint64_t>(batch->rows) * a.parts;
     return launch(rt, "xpu_cache8_append" + form_of(cache->dtype, cache->head_dim),
-                  std::min<uint64_t>((waves + 3) / 4, rt->compute_units * 8ull), a);
+                  std::min<uint64_t>((waves + 3) / 4, rt->compute_units * 64ull), a);
   });
 }
 
@@ -193,7 +194,7 @@ int xpu_tree_attention8_workspace(const xpu_runtime *rt, const xpu_cache8 *cache
     if (int rc = check_heads(name, heads, cache->kv_heads, 1.0f)) return rc;
     if (int rc = check_runtime(name, rt)) return rc;
     *bytes = batch->rows && batch->n_seqs
-                 ? tree_plan(*rt, cache->kv_heads, cache->page_size, cache->head_dim, *batch, heads).bytes
+                 ? tree_plan(*rt, true, cache->kv_heads, cache->page_size, cache->head_dim, *batch, heads).bytes
                  : 0;
     return XPU_OK;
   });
@@ -212,7 +213,7 @@ int xpu_tree_attention8(xpu_runtime *rt, const xpu_cache8 *cache, const xpu_batc
     const TreeRows rows{heads, scale, q, q_stride, visible, out, out_stride, workspace, workspace_bytes};
     if (int rc = check_tree_rows(name, rows, *batch, cache->head_dim)) return rc;
     if (int rc = check_runtime(name, rt)) return rc;
-    return launch_tree(name, rt, "xpu_tree_attention8", pool8_of(*cache, layer), cache->dtype, cache->head_dim, *batch,
+    return launch_tree(name, rt, true, pool8_of(*cache, layer), cache->dtype, cache->head_dim, *batch,
                        rows);
   });
 }
@@ -225,8 +226,12 @@ int xpu_cache8_keep(xpu_runtime *rt, const xpu_cache8 *cache, const xpu_batch *b
     if (int rc = check_keep(name, batch, kept, counts, new_context)) return rc;
     if (int rc = check_runtime(name, rt)) return rc;
     if (!batch->n_seqs) return XPU_OK;
-    const xpu::KeepArgs a{pool8_of(*cache, 0), batch_of(*batch), kept, counts, new_context};
-    const uint64_t groups = (static_cast<uint64_t>(cache->layers) * cache->kv_heads * 2 + 3) / 4;
+    xpu::Keep8Args a{{pool8_of(*cache, 0), batch_of(*batch), kept, counts, new_context}, 1};
+    uint64_t groups = static_cast<uint64_t>(cache->layers) * cache->kv_heads * 2;
+    if (groups * batch->n_seqs > rt->compute_units * 8ull) {  // more blocks than run at once
+      a.per_block = 4;
+      groups = (groups + 3) / 4;
+    }
     return launch(rt, cache->head_dim == 128 ? "xpu_cache8_keep_d128" : "xpu_cache8_keep_d64", batch->n_seqs * groups, a);
   });
 }

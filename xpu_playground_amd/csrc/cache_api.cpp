@@ -40,7 +40,7 @@ int xpu_tree_attention_workspace(const xpu_runtime *rt, const xpu_cache *cache, 
     if (int rc = check_batch(name, batch, false)) return rc;
     if (int rc = check_heads(name, heads, cache->kv_heads, 1.0f)) return rc;
     if (int rc = check_runtime(name, rt)) return rc;
-    *bytes = batch->rows && batch->n_seqs ? tree_plan(*rt, cache->kv_heads, cache->page_size, cache->head_dim, *batch, heads).bytes : 0;
+    *bytes = batch->rows && batch->n_seqs ? tree_plan(*rt, false, cache->kv_heads, cache->page_size, cache->head_dim, *batch, heads).bytes : 0;
     return XPU_OK;
   });
 }
@@ -61,7 +61,7 @@ int xpu_tree_attention(xpu_runtime *rt, const xpu_cache *cache, const xpu_batch 
     xpu::PoolArgs pool = pool_of(*cache);
     pool.k += layer * cache->layer_stride;
     pool.v += layer * cache->layer_stride;
-    return launch_tree(name, rt, "xpu_tree_attention", pool, cache->dtype, cache->head_dim, *batch, rows);
+    return launch_tree(name, rt, false, pool, cache->dtype, cache->head_dim, *batch, rows);
   });
 }
 

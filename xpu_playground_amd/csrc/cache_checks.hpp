@@ -198,15 +198,16 @@ struct TreePlan {
   uint32_t join_waves = 1; // so many wavefronts
 };
 
-inline TreePlan tree_plan(const xpu_runtime &rt, uint32_t kv_heads, uint32_t page_size, uint32_t head_dim,
+// `eight`: over 8-bit pages (kernels/tree_attention8.hip).
+inline TreePlan tree_plan(const xpu_runtime &rt, bool eight, uint32_t kv_heads, uint32_t page_size, uint32_t head_dim,
                           const xpu_batch &b, uint32_t heads) {
   TreePlan p;
   const uint64_t rows = static_cast<uint64_t>(b.rows) * (heads / kv_heads);
-  // 64 rows per block where sequences have more than 22 rows on average, so
+  // 16 bits: 64 rows per block where sequences have more than 22 rows on average, so
   // that the larger ones do not read their keys twice (48 ragged sequences of
   // 1 .. 26 nodes x 4 heads, 28 rows on average, 98.4 us in 32s and 90.5 in
   // 64s; 23 rows 93.8 and 90.5; 20 rows 86.8 and 88.2; 4 rows 69.5 and 72.7)
-  p.sub_tiles = rows > 22ull * b.n_seqs ? 2 : 1;
+  p.sub_tiles = !eight && rows > 22ull * b.n_seqs ? 2 : 1;
   const uint64_t row_tiles = rows / (32 * p.sub_tiles) + b.n_seqs;  // at most
   const uint64_t tiles = (static_cast<uint64_t>(b.table_pitch) * page_size + 31) / 32;
   const bool cut = tiles > p.least;
@@ -219,10 +220,13 @@ inline TreePlan tree_plan(const xpu_runtime &rt, uint32_t kv_heads, uint32_t pag
   // positions 28.1 and 31.5, behind 16000 19.2 and 23.6). Where more than four
   // fifths of them are row tiles, the chunks get too uneven: three per unit (48
   // single tokens 70.0 us, and 79.8 cut to fit; 32 drafts of up to 8 nodes 53.4
-  // to fit and 56.0).
-  const uint64_t fit = 2 * rt.compute_units / kv_heads;
+  // to fit and 56.0). Over 8-bit pages a unit holds three blocks of 32 rows (the
+  // four drafts 297 us, cut for two 345; 48 single tokens 39.5 and 42.5; in 64s,
+  // which leave room for two, 313 and 63), and two per unit do where they do not
+  // fit (48 of 1 .. 26 nodes 46.5 us, with three 51.0).
+  const uint64_t fit = (eight ? 3 : 2) * rt.compute_units / kv_heads;
   if (cut && b.n_seqs <= 64 && row_tiles <= fit * 4 / 5) p.fit = static_cast<uint32_t>(fit);
-  p.target = std::max(1u, 3 * rt.compute_units / kv_heads);
+  p.target = std::max(1u, (eight ? 2 : 3) * rt.compute_units / kv_heads);
   p.slots = p.fit ? fit : row_tiles + (cut ? p.target : 0);
   p.bytes = cut ? p.slots * kv_heads * (32ull * p.sub_tiles * (head_dim + 2)) * 4 : 0;
   // the fewer joins, the more wavefronts for each, which read its chunks side
@@ -263,11 +267,10 @@ inline int check_tree_rows(const char *name, const TreeRows &r, const xpu_batch 
   return XPU_OK;
 }
 
-// `pool`: the layer's pages; `kernel`: the name that the kernels of one page
-// format begin with.
-inline int launch_tree(const char *name, xpu_runtime *rt, const std::string &kernel, const PoolArgs &pool, int32_t dtype,
+// `pool`: the layer's pages.
+inline int launch_tree(const char *name, xpu_runtime *rt, bool eight, const PoolArgs &pool, int32_t dtype,
                        uint32_t head_dim, const xpu_batch &b, const TreeRows &r) {
-  const TreePlan plan = tree_plan(*rt, pool.kv_heads, pool.page_size, head_dim, b, r.heads);
+  const TreePlan plan = tree_plan(*rt, eight, pool.kv_heads, pool.page_size, head_dim, b, r.heads);
   if (plan.bytes && (!r.workspace || !aligned(r.workspace, 16) || r.workspace_bytes < plan.bytes))
     return invalid(name, "needs a workspace of " + std::to_string(plan.bytes) + " bytes, 16-byte aligned");
   TreeArgs a{};
@@ -287,7 +290,8 @@ inline int launch_tree(const char *name, xpu_runtime *rt, const std::string &ker
   a.scale_log2e = static_cast<float>(r.scale * kLog2e);
   const std::string form =
       std::string("_") + type_name(dtype) + "_d" + std::to_string(head_dim) + "_r" + std::to_string(plan.sub_tiles);
-  if (int rc = launch(rt, kernel + form, plan.slots * pool.kv_heads, a)) return rc;
+  if (int rc = launch(rt, (eight ? "xpu_tree_attention8" : "xpu_tree_attention") + form, plan.slots * pool.kv_heads, a))
+    return rc;
   if (!plan.bytes) return XPU_OK;
   const std::string join = "xpu_tree_join" + form + "_w" + std::to_string(plan.join_waves);
   return plan.join_waves > 1 ? launch(rt, join, plan.joins, a, 1, nullptr, 64 * plan.join_waves)

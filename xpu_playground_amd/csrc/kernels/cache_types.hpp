@@ -93,6 +93,11 @@ struct KeepArgs {
   uint32_t *new_context;
 };
 
+struct Keep8Args {
+  KeepArgs keep;
+  uint32_t per_block;  // parts (layer, kv head, K or V) that a block takes: 1 or 4
+};
+
 // The rotation of rows on their way (half = rotated dims / 2; 0: none).
 struct RotaryArgs {
   const float *cos, *sin;  // [positions][half]

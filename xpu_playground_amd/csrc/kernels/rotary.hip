@@ -86,13 +86,16 @@ template <int DT, int D> XPU_DEVICE void turn(float (&x)[8], const RotaryArgs &r
     const bool low = dim < r.half;
     const uint32_t step = r.half / 8u;
     const int partner = static_cast<int>(dim >= 2u * r.half ? lane : low ? lane + step : lane - step);
+    const bool row = D == 128 && r.half == 64;  // the other half of a row of 16 lanes
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
-      const float other = __shfl(x[i], partner), s = low ? -a.s[i] : a.s[i];
+      const float other = row ? xor8_f(x[i]) : __shfl(x[i], partner), s = low ? -a.s[i] : a.s[i];
       if (dim < 2u * r.half) x[i] = x[i] * a.c[i] + other * s;
     }
   }
 }
+
+constexpr uint32_t kAhead = 4;  // a wavefront's loads of rows on their way
 
 template <int DT> XPU_DEVICE u32x4 pack8(const float (&x)[8]) {
   return u32x4{dma::cvt_pack<DT>(x[0], x[1]), dma::cvt_pack<DT>(x[2], x[3]), dma::cvt_pack<DT>(x[4], x[5]),
@@ -122,15 +125,23 @@ template <int DT, int D> XPU_DEVICE void turn_q(const RotateArgs &a, uint32_t ro
   const bool known = a.rot.half == 0 || at.turned < a.rot.positions;
   if (!known) report(a.pool);
   const Angles angles = angles_of<D>(a.rot, at.turned);
-  const uint32_t lane = lane_id(), dim = lane % kGroup * 8u;
-  for (uint32_t h0 = part * kPer; h0 < a.heads; h0 += a.parts * kPer) {
-    const uint32_t head = h0 + lane / kGroup, from = min(head, a.heads - 1u) * D + dim;
-    float x[8];
-    unpack8<DT>(*reinterpret_cast<const u32x4 *>(a.q + row * a.q_stride + from), x);
-    turn<DT, D>(x, a.rot, angles, a.rot.q_gain);
+  const uint32_t lane = lane_id(), dim = lane % kGroup * 8u, step = a.parts * kPer;
+  for (uint32_t h0 = part * kPer; h0 < a.heads; h0 += kAhead * step) {
+    auto head = [&](uint32_t j) { return h0 + j * step + lane / kGroup; };
+    auto at_of = [&](uint32_t j) { return min(head(j), a.heads - 1u) * D + dim; };
+    u32x4 raw[kAhead];
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) x[i] = known ? x[i] : __builtin_nanf("");
-    if (head < a.heads) *reinterpret_cast<u32x4 *>(a.q_out + row * a.out_stride + from) = pack8<DT>(x);
+    for (uint32_t j = 0; j < kAhead; ++j) raw[j] = *reinterpret_cast<const u32x4 *>(a.q + row * a.q_stride + at_of(j));
+#pragma unroll
+    for (uint32_t j = 0; j < kAhead; ++j) {
+      if (h0 + j * step >= a.heads) break;
+      float x[8];
+      unpack8<DT>(raw[j], x);
+      turn<DT, D>(x, a.rot, angles, a.rot.q_gain);
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) x[i] = known ? x[i] : __builtin_nanf("");
+      if (head(j) < a.heads) *reinterpret_cast<u32x4 *>(a.q_out + row * a.out_stride + at_of(j)) = pack8<DT>(x);
+    }
   }
 }
 
@@ -149,22 +160,38 @@ template <int DT, int D> XPU_DEVICE void append_rotary(const RotateArgs &a) {
                                       a.batch.table_pitch, at.pos, D);
     if (!known || place == kNowhere) report(a.pool);
     const Angles angles = angles_of<D>(a.rot, at.turned);
-    for (uint32_t u0 = part * kPer; u0 < total; u0 += a.parts * kPer) {
-      const uint32_t unit = u0 + lane / kGroup, in = min(unit, total - 1u);
-      const bool is_q = in < a.heads, is_v = in >= a.heads + kv;
-      const uint32_t head = is_q ? in : (in - a.heads) % kv;
-      const uint16_t *from = is_q ? a.q + row * a.q_stride : is_v ? a.v + row * a.v_stride : a.k + row * a.k_stride;
-      const u32x4 raw = *reinterpret_cast<const u32x4 *>(from + head * D + dim);
-      float x[8];
-      unpack8<DT>(raw, x);
-      turn<DT, D>(x, a.rot, angles, is_q ? a.rot.q_gain : is_v ? nullptr : a.rot.k_gain);
+    const uint32_t step = a.parts * kPer;
+    for (uint32_t u0 = part * kPer; u0 < total; u0 += kAhead * step) {
+      struct Unit {
+        bool is_q, is_v;
+        uint32_t head;
+      };
+      auto unit_of = [&](uint32_t j) {
+        const uint32_t in = min(u0 + j * step + lane / kGroup, total - 1u);
+        return Unit{in < a.heads, in >= a.heads + kv, in < a.heads ? in : (in - a.heads) % kv};
+      };
+      u32x4 raw[kAhead];
 #pragma unroll
-      for (uint32_t i = 0; i < 8; ++i) x[i] = known ? x[i] : __builtin_nanf("");
-      const u32x4 y = is_v ? raw : pack8<DT>(x);
-      if (unit >= total || (!is_q && (!known || place == kNowhere))) continue;
-      uint16_t *to = is_q ? a.q_out + row * a.out_stride + head * D
-                          : (is_v ? a.pool.v : a.pool.k) + place + static_cast<uint64_t>(head) * a.pool.page_size * D;
-      *reinterpret_cast<u32x4 *>(to + dim) = y;
+      for (uint32_t j = 0; j < kAhead; ++j) {
+        const Unit u = unit_of(j);
+        const uint16_t *from = u.is_q ? a.q + row * a.q_stride : u.is_v ? a.v + row * a.v_stride : a.k + row * a.k_stride;
+        raw[j] = *reinterpret_cast<const u32x4 *>(from + u.head * D + dim);
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < kAhead; ++j) {
+        if (u0 + j * step >= total) break;
+        const Unit u = unit_of(j);
+        float x[8];
+        unpack8<DT>(raw[j], x);
+        turn<DT, D>(x, a.rot, angles, u.is_q ? a.rot.q_gain : u.is_v ? nullptr : a.rot.k_gain);
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) x[i] = known ? x[i] : __builtin_nanf("");
+        const u32x4 y = u.is_v ? raw[j] : pack8<DT>(x);
+        if (u0 + j * step + lane / kGroup >= total || (!u.is_q && (!known || place == kNowhere))) continue;
+        uint16_t *to = u.is_q ? a.q_out + row * a.out_stride + u.head * D
+                              : (u.is_v ? a.pool.v : a.pool.k) + place + static_cast<uint64_t>(u.head) * a.pool.page_size * D;
+        *reinterpret_cast<u32x4 *>(to + dim) = y;
+      }
     }
   }
 }

@@ -139,64 +139,69 @@ template <int D, int R> constexpr uint32_t kPartial = 32u * R * (D + 2u);
 // adds up a quarter of the columns (kMine registers of every lane's D / 2),
 // in the order of the keys. A side without a finite score has only zeros or
 // NaN in its sum, which stay. `bad` makes the rows NaN.
-// po: D / 2 columns of 64 floats per wavefront, meet: 128 floats per wavefront.
-template <int DT, int D, int R>
+// po: D / 2 / PASSES columns of 64 floats per wavefront (so many passes over the
+// columns), meet: 128 floats per wavefront.
+template <int DT, int D, int R, int PASSES = 1>
 XPU_DEVICE void finish(const TreeArgs &a, const Rows<DT, D, R> &rows, const Place &place, const uint64_t (&sees)[R],
                        uint32_t item, bool bad, float *po, float *meet) {
   const uint32_t lane = lane_id(), hh = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t kvh = blockIdx.x % a.pool.kv_heads, group = a.heads / a.pool.kv_heads;
   const Sequence &s = place.s;
   const uint32_t row_tile = (item - place.first) % s.row_tiles, rows_in = min(s.n * group - row_tile * 32u * R, 32u * R);
-  constexpr uint32_t kMine = D / 8;
+  constexpr uint32_t kColumns = D / 2 / PASSES, kMine = kColumns / 4;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    __syncthreads();  // the tiles, the queries, the sub-tile before are read
-    meet[(wave * 2u) * 64u + lane] = rows.m[r];
-    meet[(wave * 2u + 1u) * 64u + lane] = bad ? __builtin_nanf("") : rows.total(r);
 #pragma unroll
-    for (uint32_t dt = 0; dt < D / 32; ++dt)
+    for (uint32_t pass = 0; pass < PASSES; ++pass) {
+      __syncthreads();  // the tiles, the queries, the columns before are read
+      if (pass == 0) {
+        meet[(wave * 2u) * 64u + lane] = rows.m[r];
+        meet[(wave * 2u + 1u) * 64u + lane] = bad ? __builtin_nanf("") : rows.total(r);
+      }
 #pragma unroll
-      for (uint32_t i = 0; i < 16; ++i) po[(wave * (D / 2u) + dt * 16u + i) * 64u + lane] = rows.o[r][dt][i];
-    __syncthreads();
-    const float ninf = -__builtin_inff();
-    float m[4], x[4], top = ninf, sum = 0.0f;
+      for (uint32_t c = 0; c < kColumns; ++c)
+        po[(wave * kColumns + c) * 64u + lane] = rows.o[r][(pass * kColumns + c) / 16u][(pass * kColumns + c) % 16u];
+      __syncthreads();
+      const float ninf = -__builtin_inff();
+      float m[4], x[4], top = ninf, sum = 0.0f;
 #pragma unroll
-    for (uint32_t w = 0; w < 4; ++w) top = fmaxf(top, m[w] = meet[w * 128u + lane]);
+      for (uint32_t w = 0; w < 4; ++w) top = fmaxf(top, m[w] = meet[w * 128u + lane]);
 #pragma unroll
-    for (uint32_t w = 0; w < 4; ++w) {
-      const float side = meet[w * 128u + 64u + lane];
-      x[w] = m[w] == ninf ? 0.0f : __builtin_amdgcn_exp2f((m[w] - top) * a.scale_log2e);
-      sum += m[w] == ninf ? side : side * x[w];
-    }
-    float o[kMine];
+      for (uint32_t w = 0; w < 4; ++w) {
+        const float side = meet[w * 128u + 64u + lane];
+        x[w] = m[w] == ninf ? 0.0f : __builtin_amdgcn_exp2f((m[w] - top) * a.scale_log2e);
+        sum += m[w] == ninf ? side : side * x[w];
+      }
+      float o[kMine];
 #pragma unroll
-    for (uint32_t i = 0; i < kMine; ++i) {
-      o[i] = 0.0f;
+      for (uint32_t i = 0; i < kMine; ++i) {
+        o[i] = 0.0f;
 #pragma unroll
-      for (uint32_t w = 0; w < 4; ++w)
-        o[i] = __builtin_fmaf(po[(w * (D / 2u) + wave * kMine + i) * 64u + lane], x[w], o[i]);
-    }
-    // register wave * kMine + i: dims 32 (reg / 16) + 8 (reg % 16 / 4) + 4 hh + reg % 4
-    const uint32_t in = 32u * r + (lane & 31u), row = row_tile * 32u * R + in;
-    const uint32_t dim = wave * 2u * kMine + 4u * hh;
-    if (in >= rows_in) continue;
-    if (place.chunks == 1) {
-      // (the sum has the NaN of every wavefront that met a missing page)
-      const bool empty = s.context == 0 && a.visible && sees[r] == 0 && sum == 0.0f;
-      const float by = empty ? 0.0f : 1.0f / sum;
-      uint16_t *to = a.out + (s.first + row / group) * a.out_stride + (kvh * group + row % group) * D + dim;
+        for (uint32_t w = 0; w < 4; ++w)
+          o[i] = __builtin_fmaf(po[(w * kColumns + wave * kMine + i) * 64u + lane], x[w], o[i]);
+      }
+      // register pass * kColumns + wave * kMine + i: dims 32 (reg / 16) + 8 (reg % 16 / 4) + 4 hh + reg % 4
+      const uint32_t in = 32u * r + (lane & 31u), row = row_tile * 32u * R + in;
+      const uint32_t dim = 2u * (pass * kColumns + wave * kMine) + 4u * hh;
+      if (in >= rows_in) continue;
+      if (place.chunks == 1) {
+        // (the sum has the NaN of every wavefront that met a missing page)
+        const bool empty = s.context == 0 && a.visible && sees[r] == 0 && sum == 0.0f;
+        const float by = empty ? 0.0f : 1.0f / sum;
+        uint16_t *to = a.out + (s.first + row / group) * a.out_stride + (kvh * group + row % group) * D + dim;
 #pragma unroll
-      for (uint32_t w = 0; w < kMine / 4; ++w)
-        *reinterpret_cast<u32x2 *>(to + 8u * w) = u32x2{dma::cvt_pack<DT>(o[4 * w] * by, o[4 * w + 1] * by),
-                                                        dma::cvt_pack<DT>(o[4 * w + 2] * by, o[4 * w + 3] * by)};
-    } else {
-      float *slot = a.partial + (static_cast<uint64_t>(item) * a.pool.kv_heads + kvh) * kPartial<D, R>;
-      float *to = slot + in * D + dim;
+        for (uint32_t w = 0; w < kMine / 4; ++w)
+          *reinterpret_cast<u32x2 *>(to + 8u * w) = u32x2{dma::cvt_pack<DT>(o[4 * w] * by, o[4 * w + 1] * by),
+                                                          dma::cvt_pack<DT>(o[4 * w + 2] * by, o[4 * w + 3] * by)};
+      } else {
+        float *slot = a.partial + (static_cast<uint64_t>(item) * a.pool.kv_heads + kvh) * kPartial<D, R>;
+        float *to = slot + in * D + dim;
 #pragma unroll
-      for (uint32_t w = 0; w < kMine / 4; ++w)
-        *reinterpret_cast<dma::f32x4 *>(to + 8u * w) = dma::f32x4{o[4 * w], o[4 * w + 1], o[4 * w + 2], o[4 * w + 3]};
-      if (wave == 0 && hh == 0)
-        *reinterpret_cast<dma::f32x2 *>(slot + 32u * R * D + 2u * in) = dma::f32x2{top, sum};
+        for (uint32_t w = 0; w < kMine / 4; ++w)
+          *reinterpret_cast<dma::f32x4 *>(to + 8u * w) = dma::f32x4{o[4 * w], o[4 * w + 1], o[4 * w + 2], o[4 * w + 3]};
+        if (pass == 0 && wave == 0 && hh == 0)
+          *reinterpret_cast<dma::f32x2 *>(slot + 32u * R * D + 2u * in) = dma::f32x2{top, sum};
+      }
     }
   }
 }
