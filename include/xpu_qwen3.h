@@ -1,5 +1,5 @@
 /*
- * xpu_qwen3.h - batch-1 greedy Qwen3 decode on gfx950 (C ABI).
+ * xpu_qwen3.h - batch-1 Qwen3 decode on gfx950 (C ABI), greedy or sampled.
  *
  * Replaces the reference engine qwen3/main.cpp:118-329 (Engine: weight
  * arena, KV caches, RoPE tables, decode(token, position)) and its command
@@ -141,6 +141,17 @@ int xpu_qwen3_set_prefill(xpu_qwen3 *eng, int mode);
  * per head. XPU_ERR_INVALID when the module lacks the kernels. */
 int xpu_qwen3_set_attention_split(xpu_qwen3 *eng, uint32_t min_context);
 
+/* Sampling in xpu_qwen3_generate, any mode: each new token is drawn from its
+ * step's logits by xpu_sample (xpu_sample.h says what temperature, top_k, top_p
+ * and min_p keep; 0, 1 and 0 filter nothing) with the random number that a
+ * counter hash gives for (seed, the position before the token), so a
+ * continuation with the same seed draws what one call would have. Temperature 0
+ * (the default) takes the argmax and ignores the others but for their ranges;
+ * XPU_ERR_INVALID for a temperature that is negative or not finite, a negative
+ * top_p, a min_p outside [0, 1], NaN, or a vocabulary above 2^20. The first call
+ * with a temperature allocates. The reference is greedy only. */
+int xpu_qwen3_set_sampling(xpu_qwen3 *eng, float temperature, uint32_t top_k, float top_p, float min_p, uint64_t seed);
+
 /* One forward step at `position` for input `token`; *next = greedy token
  * (Engine::decode, main.cpp:159-226). A non-finite logit fails with
  * XPU_ERR_VERIFY ("model produced a NaN or infinity", main.cpp:223-224). */
@@ -150,9 +161,9 @@ int xpu_qwen3_decode(xpu_qwen3 *eng, uint32_t token, uint32_t position, uint32_t
 int xpu_qwen3_logits(xpu_qwen3 *eng, uint16_t *out, uint64_t count);
 int xpu_qwen3_hidden(xpu_qwen3 *eng, uint16_t *out, uint64_t count);
 
-/* Prompt + greedy loop (main.cpp:342-352): the prompt goes through decode one
+/* Prompt + decode loop (main.cpp:342-352), greedy or sampled (xpu_qwen3_set_sampling): the prompt goes through decode one
  * position at a time (or the batched forms, xpu_qwen3_set_prefill); token i
- * of out is the argmax after position n_prompt - 1 + i; stops after an EOS id (151645, 151643) when
+ * of out is the one after position n_prompt - 1 + i; stops after an EOS id (151645, 151643) when
  * stop_on_eos. *n_out = number of ids written. prompt_ms / decode_ms (may be
  * NULL): device time of the prompt steps and of the n_out - 1 decode steps. */
 int xpu_qwen3_generate(xpu_qwen3 *eng, const uint32_t *prompt, uint32_t n_prompt, uint32_t max_new,
@@ -163,6 +174,7 @@ int xpu_qwen3_generate(xpu_qwen3 *eng, const uint32_t *prompt, uint32_t n_prompt
  *   --model-dir DIR | --synthetic PRESET [--seed N] [--gain-std X]
  *   --input-ids FILE|- --max-new-tokens N [--max-seq-len N]
  *   [--mode graph|eager|reference] [--prefill batched|gemm|stepwise] [--no-eos-stop]
+ *   [--temperature X [--top-k N] [--top-p X] [--min-p X] [--sample-seed N]]
  * prints {"generated_ids":[...]} on stdout, diagnostics on stderr. */
 int run_qwen3(int argc, char **argv);
 

@@ -15,6 +15,7 @@
 //                           (gate/up stored as one [gate; up] matrix)
 //   xpu_q3_norm_gemv_logits final RMSNorm + tied lm_head + per-block argmax
 //   xpu_q3_argmax_finish    argmax, next token, position advance
+//   xpu_q3_take_token       a drawn token in place of the argmax
 // The decode position and token live in device memory (state[0], state[1])
 // so one captured graph serves every step. Engine caches: K and V
 // chunk-major [kv_head][16][max_seq][8] (eight-element chunk j of every
@@ -1159,6 +1160,13 @@ extern "C" __global__ __launch_bounds__(1024) void xpu_q3_argmax_finish(
       if (g < gen_capacity) gen[g] = token;
     }
   }
+}
+
+// A drawn token gen[index] (xpu_sample wrote it there over the argmax) as the
+// next step's input, behind xpu_q3_argmax_finish.
+extern "C" __global__ __launch_bounds__(64) void xpu_q3_take_token(uint32_t *state, const uint32_t *__restrict__ gen,
+                                                                    uint32_t index) {
+  if (threadIdx.x == 0) state[1] = state[2] = gen[index];
 }
 
 // ------------------------------------------------------------ batched prefill

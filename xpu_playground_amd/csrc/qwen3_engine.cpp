@@ -1,4 +1,4 @@
-// Qwen3 batch-1 greedy decode engine on gfx950 (include/xpu_qwen3.h).
+// Qwen3 batch-1 decode engine on gfx950 (include/xpu_qwen3.h).
 //
 // Reference: qwen3/main.cpp:118-329 (Engine) and :17-102,333-363 (command
 // line); checkpoint validation qwen3/model.cpp:376-495. The reference engine
@@ -16,6 +16,7 @@
 // [layer][max_seq][kv_head][128] for both).
 #include "../../include/xpu_qwen3.h"
 #include "../../include/xpu_kernels.h"
+#include "../../include/xpu_sample.h"
 #include "host_common.hpp"
 #include "json.hpp"
 #include "runtime_internal.hpp"
@@ -187,13 +188,22 @@ struct xpu_qwen3 {
     const xpu::KernelInfo *k = nullptr;
     uint32_t block = 0;
   } pf_qkv_m, pf_o_m, pf_gu_m, pf_down_m;
+  // sampling in generate (xpu_qwen3_set_sampling): one block, allocated by
+  // the first call; draws[p] is the random number behind position p
+  bool sampling = false;
+  void *sample_block = nullptr;
+  xpu_sampling sample{};
+  void *sample_workspace = nullptr;
+  uint64_t sample_bytes = 0;
+  Launch take_l;
 
   ~xpu_qwen3() {
     if (graph) xpu_rt_graph_destroy(graph);
     if (graph_split) xpu_rt_graph_destroy(graph_split);
     if (rt) {
       for (void *p : {static_cast<void *>(arena), static_cast<void *>(kcache), static_cast<void *>(vcache),
-                      static_cast<void *>(cos_t), static_cast<void *>(sin_t), static_cast<void *>(x), pf_block})
+                      static_cast<void *>(cos_t), static_cast<void *>(sin_t), static_cast<void *>(x), pf_block,
+                      sample_block})
         if (p) xpu_rt_free(rt, p);
       if (owns_rt) xpu_rt_destroy(rt);
     }
@@ -1263,6 +1273,76 @@ extern "C" int xpu_qwen3_set_attention_split(xpu_qwen3 *eng, uint32_t min_contex
   return XPU_OK;
 }
 
+extern "C" int xpu_qwen3_set_sampling(xpu_qwen3 *eng, float temperature, uint32_t top_k, float top_p, float min_p,
+                                      uint64_t seed) {
+  if (!(temperature >= 0.0f && temperature <= 3.402823466e38f))
+    return set_error(XPU_ERR_INVALID, "temperature must be 0 or more, and finite");
+  if (!(top_p >= 0.0f)) return set_error(XPU_ERR_INVALID, "top_p must be 0 or more");
+  if (!(min_p >= 0.0f && min_p <= 1.0f)) return set_error(XPU_ERR_INVALID, "min_p must be in [0, 1]");
+  if (!eng) return set_error(XPU_ERR_INVALID, "null engine");
+  if (temperature == 0.0f) {
+    eng->sampling = false;
+    return XPU_OK;
+  }
+  return xpu::guarded("xpu_qwen3_set_sampling", [&]() -> int {
+    xpu_qwen3 &e = *eng;
+    e.sampling = false;  // until everything is there
+    e.take_l.k = e.rt->find_exact("xpu_q3_take_token");
+    e.take_l.grid = 1;
+    if (!e.take_l.k) return set_error(XPU_ERR_INVALID, "the module has no kernels for sampling");
+    xpu_sampling s{};
+    s.dtype = XPU_DTYPE_BF16;
+    s.rows = 1;
+    s.vocab = e.c.vocab;
+    s.stride = e.c.vocab;
+    uint64_t bytes = 0;
+    int rc = xpu_sample_workspace(e.rt, &s, &bytes);
+    if (rc) return rc;
+    const uint64_t draws = (e.max_seq * 4ull + 255) & ~uint64_t{255};
+    if (!e.sample_block && (rc = xpu_rt_alloc(e.rt, 256 + draws + bytes, 256, &e.sample_block))) return rc;
+    std::vector<uint32_t> words(64 + draws / 4);
+    std::memcpy(&words[0], &temperature, 4);
+    words[1] = top_k;
+    std::memcpy(&words[2], &top_p, 4);
+    std::memcpy(&words[3], &min_p, 4);
+    for (uint32_t p = 0; p < e.max_seq; ++p) {
+      const float u = static_cast<float>(xpu::counter_hash(seed, p) >> 40) * 0x1p-24f;
+      std::memcpy(&words[64 + p], &u, 4);
+    }
+    if ((rc = xpu_rt_copy_to_device(e.rt, e.sample_block, words.data(), words.size() * 4))) return rc;
+    const float *at = static_cast<const float *>(e.sample_block);
+    s.temperature = at;
+    s.top_k = reinterpret_cast<const uint32_t *>(at + 1);
+    s.top_p = at + 2;
+    s.min_p = at + 3;
+    s.random = at + 64;
+    e.sample = s;
+    e.sample_workspace = static_cast<uint8_t *>(e.sample_block) + 256 + draws;
+    e.sample_bytes = bytes;
+    e.sampling = true;
+    return XPU_OK;
+  });
+}
+
+namespace {
+
+// With sampling: draws generated token `index`, the one behind `position`, of
+// the step's logits into gen.
+int draw_token(xpu_qwen3 &e, uint32_t position, uint32_t index) {
+  xpu_sampling s = e.sample;
+  s.random += position;
+  return xpu_sample(e.rt, &s, e.logits, e.gen + index, nullptr, e.sample_workspace, e.sample_bytes);
+}
+
+// The same behind a fused step, whose argmax it replaces.
+int replace_token(xpu_qwen3 &e, uint32_t position, uint32_t index) {
+  if (!e.sampling) return XPU_OK;
+  const int rc = draw_token(e, position, index);
+  return rc ? rc : launch(e, e.take_l, 64, {{8, &e.state}, {8, &e.gen}, {4, &index}});
+}
+
+}  // namespace
+
 namespace {
 
 // The reference-mode kernels keep the caches position-major, the fused ones
@@ -1338,14 +1418,26 @@ extern "C" int xpu_qwen3_generate(xpu_qwen3 *eng, const uint32_t *prompt, uint32
   if (eng->mode == XPU_QWEN3_REFERENCE) {
     auto t0 = std::chrono::steady_clock::now();
     uint32_t next = 0;
+    auto draw = [&](uint32_t index) {
+      if (!eng->sampling) return XPU_OK;
+      int failed = draw_token(*eng, n_prompt - 1 + index, index);
+      if (!failed) failed = xpu_rt_copy_from_device(eng->rt, &next, eng->gen + index, 4);
+      return failed || next != XPU_SAMPLE_NONE
+                 ? failed
+                 : set_error(XPU_ERR_VERIFY, "model produced a NaN or infinity in vocabulary logits");
+    };
     for (uint32_t p = 0; p < n_prompt; ++p)
       if ((rc = xpu_qwen3_decode(eng, prompt[p], p, &next))) return rc;
+    if ((rc = draw(0))) return rc;
     auto t1 = std::chrono::steady_clock::now();
     uint32_t produced = 0;
     for (uint32_t i = 0; i < max_new; ++i) {
       gen[produced++] = next;
       if (stop_on_eos && (next == kEos || next == kEndOfTurn)) break;
-      if (i + 1 != max_new && (rc = xpu_qwen3_decode(eng, next, n_prompt + i, &next))) return rc;
+      if (i + 1 != max_new) {
+        if ((rc = xpu_qwen3_decode(eng, next, n_prompt + i, &next))) return rc;
+        if ((rc = draw(i + 1))) return rc;
+      }
     }
     auto t2 = std::chrono::steady_clock::now();
     p_ms = std::chrono::duration<double, std::milli>(t1 - t0).count();
@@ -1367,9 +1459,11 @@ extern "C" int xpu_qwen3_generate(xpu_qwen3 *eng, const uint32_t *prompt, uint32
       if ((rc = xpu_rt_event_create(eng->rt, &v))) return rc;
     rc = xpu_rt_event_record(eng->rt, ev[0]);
     if (!rc && whole) rc = run_prefill(*eng, n_prompt, true);
+    if (!rc && whole) rc = replace_token(*eng, n_prompt - 1, 0);
     if (!rc && whole) rc = xpu_rt_event_record(eng->rt, ev[1]);
     for (uint32_t s = whole ? n_prompt : first; !rc && s < steps; ++s) {
       rc = run_fused_step(*eng, s);
+      if (!rc && s + 1 >= n_prompt) rc = replace_token(*eng, s, s + 1 - n_prompt);
       if (!rc && s + 1 == n_prompt) rc = xpu_rt_event_record(eng->rt, ev[1]);
     }
     if (!rc) rc = xpu_rt_event_record(eng->rt, ev[2]);
@@ -1407,6 +1501,10 @@ struct QwenOptions {
   float gain_std = 0.0f;
   int mode = XPU_QWEN3_GRAPH;
   int prefill = -1;  // -1: the engine's default
+  float temperature = 0.0f, top_p = 1.0f, min_p = 0.0f;
+  uint32_t top_k = 0;
+  uint64_t sample_seed = 0;
+  std::string sampling;  // the last option of sampling's own
 };
 
 [[noreturn]] void qwen_usage_error(const std::string &message) {
@@ -1428,6 +1526,17 @@ uint32_t parse_u32(const std::string &text, const std::string &option, bool allo
   return static_cast<uint32_t>(v);
 }
 
+float parse_real(const std::string &text, const std::string &option, float most) {
+  size_t used = 0;
+  float v = -1.0f;
+  try {
+    v = std::stof(text, &used);
+  } catch (...) {
+  }
+  if (used != text.size() || !(v >= 0.0f && v <= most)) qwen_usage_error("invalid value for " + option + ": " + text);
+  return v;
+}
+
 // main.cpp:43-72
 QwenOptions parse_qwen(int argc, char **argv) {
   QwenOptions o;
@@ -1437,7 +1546,8 @@ QwenOptions parse_qwen(int argc, char **argv) {
       std::cout << "Usage: " << argv[0]
                 << " --model-dir DIR | --synthetic qwen3-0.6b|qwen3-8b|tiny|small [--seed N] [--gain-std X]\n"
                    "       --input-ids FILE|- --max-new-tokens N [--max-seq-len N]\n"
-                   "       [--mode graph|eager|reference] [--prefill batched|gemm|stepwise] [--no-eos-stop]\n";
+                   "       [--mode graph|eager|reference] [--prefill batched|gemm|stepwise] [--no-eos-stop]\n"
+                   "       [--temperature X [--top-k N] [--top-p X] [--min-p X] [--sample-seed N]]\n";
       std::exit(0);
     }
     if (opt == "--no-eos-stop") { o.stop_on_eos = false; continue; }
@@ -1460,10 +1570,19 @@ QwenOptions parse_qwen(int argc, char **argv) {
       else if (v == "stepwise") o.prefill = 0;
       else if (v == "gemm") o.prefill = 2;
       else qwen_usage_error("--prefill must be batched, gemm or stepwise");
+    } else if (opt == "--temperature") {
+      o.temperature = parse_real(v, opt, 3.402823466e38f);
+    } else if (opt == "--top-k" || opt == "--top-p" || opt == "--min-p" || opt == "--sample-seed") {
+      o.sampling = opt;
+      if (opt == "--top-k") o.top_k = parse_u32(v, opt, true);
+      else if (opt == "--top-p") o.top_p = parse_real(v, opt, 3.402823466e38f);
+      else if (opt == "--min-p") o.min_p = parse_real(v, opt, 1.0f);
+      else o.sample_seed = parse_u32(v, opt, true);
     } else {
       qwen_usage_error("unknown option: " + opt);
     }
   }
+  if (o.temperature == 0.0f && !o.sampling.empty()) qwen_usage_error(o.sampling + " needs --temperature above 0");
   if (o.model_dir.empty() == o.synthetic.empty()) qwen_usage_error("exactly one of --model-dir and --synthetic is required");
   if (o.input_ids.empty()) qwen_usage_error("--input-ids is required");
   if (!o.has_max_new_tokens) qwen_usage_error("--max-new-tokens is required");
@@ -1522,6 +1641,8 @@ extern "C" int run_qwen3(int argc, char **argv) {
     const double load_s = std::chrono::duration<double>(std::chrono::steady_clock::now() - t0).count();
     if (xpu_qwen3_set_mode(eng, o.mode)) throw std::runtime_error(xpu_last_error());
     if (o.prefill >= 0 && xpu_qwen3_set_prefill(eng, o.prefill)) throw std::runtime_error(xpu_last_error());
+    if (xpu_qwen3_set_sampling(eng, o.temperature, o.top_k, o.top_p, o.min_p, o.sample_seed))
+      throw std::runtime_error(xpu_last_error());
     std::cerr << "qwen3_hip: " << eng->rt->name << " (" << eng->rt->arch << "), " << cfg.layers << " layers, hidden "
               << cfg.hidden << ", weights " << (eng->arena_bytes >> 20) << " MiB loaded in " << load_s << " s\n";
     std::vector<uint32_t> out(std::max(o.max_new_tokens, 1u));

@@ -1,8 +1,8 @@
 """Qwen3 decode engine bindings (include/xpu_qwen3.h).
 
 Engine mirrors the reference's Engine (qwen3/main.cpp:118-329): decode(token,
-position) -> next token, plus the prompt + greedy generate loop
-(main.cpp:342-352). Everything runs on the gfx950 kernels; there is no CPU
+position) -> next token, plus the prompt + generate loop
+(main.cpp:342-352), greedy or sampled. Everything runs on the gfx950 kernels; there is no CPU
 path.
 """
 from __future__ import annotations
@@ -123,6 +123,12 @@ class Engine:
         """Split the attention over compute units for contexts of at least
         min_context positions (0: never); results are bit-identical."""
         check(self.lib.xpu_qwen3_set_attention_split(self.handle, c_uint32(min_context)))
+
+    def set_sampling(self, temperature: float, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0,
+                     seed: int = 0) -> None:
+        """Draw the tokens of generate (xpu_sample with random numbers hashed
+        from seed and position); temperature 0 takes the argmax again."""
+        check(self.lib.xpu_qwen3_set_sampling(self.handle, temperature, top_k, top_p, min_p, seed))
 
     def decode(self, token: int, position: int) -> int:
         nxt = c_uint32()
