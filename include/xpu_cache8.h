@@ -12,7 +12,7 @@
  * finite values are at most 448 codes (2^-100 at least). Rows that come later
  * to a block of which the sequence has earlier rows never lower it; where they
  * raise it, the codes of the earlier rows are rounded once more to the new
- * one. A value is off by half a code's step, 2^-4 of itself and at least 2^-18
+ * one. A value is off by half a code's step, 2^-4 of itself or, if small, 2^-17
  * of the block's largest. Infinities and NaN are stored as NaN; a value whose
  * code stands for more than the largest number of `dtype` reads as infinite.
  */
