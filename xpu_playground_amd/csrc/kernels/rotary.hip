@@ -15,6 +15,11 @@
 // long as they stay normal. A wavefront takes a whole block of K or of V, so
 // the new rows' largest value is known before the first code is formed and no
 // block is written by two.
+//
+// Memory bounds both where there are many rows: 24 prompts of 17 .. 1500 rows,
+// 32 and 8 heads of size 128, 54 us in 16 bits with gains (220 MB, 4.05 TB/s),
+// 53 in 8 bits with half of the dims turned, 65 with all and gains. A step's few
+// rows are one launch and a chain of loads: 48 rows 4.4 us and 8.4, one 7.6.
 #include "cache_types.hpp"
 #include "device_common.hpp"
 
@@ -95,7 +100,9 @@ template <int DT, int D> XPU_DEVICE void turn(float (&x)[8], const RotaryArgs &r
   }
 }
 
-constexpr uint32_t kAhead = 4;  // a wavefront's loads of rows on their way
+// A wavefront's loads of rows on their way (one: the 8-bit prompts with all dims
+// and gains 71 us instead of 65; no difference in 16 bits).
+constexpr uint32_t kAhead = 4;
 
 template <int DT> XPU_DEVICE u32x4 pack8(const float (&x)[8]) {
   return u32x4{dma::cvt_pack<DT>(x[0], x[1]), dma::cvt_pack<DT>(x[2], x[3]), dma::cvt_pack<DT>(x[4], x[5]),
