@@ -2,10 +2,12 @@
 // Its parts are (layer, kv head, K or V). All kept rows of a part are loaded
 // before the first is stored, so they may move in any order. A wavefront has
 // room for 16 rows, and a block takes one part, a wavefront 16 of its rows, or,
-// where that is more blocks than the chip holds, four: up to 16 rows a wavefront's
-// own, more rows one part after the other (one sequence of 28 layers, 8 kv heads:
-// 4.9 us the first way, 7.3 the second; 48 of them 20.8 with a wavefront for up
-// to 64 rows, 13.5 so: half the registers). The rows reach at most 5 blocks of 16
+// where that is more blocks than the chip holds, as many parts as let it hold
+// all: up to 16 rows each wavefront parts of its own, more rows one part after the
+// other (one sequence of 28 layers, 8 kv heads: 4.8 us the first way, 7.3 with
+// four parts a block; 48 of them 20.8 with a wavefront for up to 64 rows, which is
+// twice the registers, 13.7 with four parts a block, 11.2 so). What is left is the
+// chain of loads: lengths, table, scale and rows. The rows reach at most 5 blocks of 16
 // positions. A block's scale becomes the largest of its own and of the scales
 // that rows bring, so codes are only ever scaled down, by powers of two; the
 // rows before the draft in its first block are rescaled with it.
@@ -18,7 +20,7 @@ namespace cache {
 template <int D> XPU_DEVICE void keep8(const KeepArgs &a, uint32_t per_block) {
   constexpr uint32_t kCpr = D / 16, kRpi = 64 / kCpr, kLoads = 16 / kRpi;
   const uint32_t lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t parts = a.pool.layers * a.pool.kv_heads * 2u, groups = per_block == 1u ? parts : (parts + 3u) / 4u;
+  const uint32_t parts = a.pool.layers * a.pool.kv_heads * 2u, groups = (parts + per_block - 1u) / per_block;
   const uint32_t seq = blockIdx.x / groups, group = blockIdx.x % groups;
   const uint32_t lo = __builtin_amdgcn_readfirstlane(a.batch.starts[seq]);
   const uint32_t hi = __builtin_amdgcn_readfirstlane(a.batch.starts[seq + 1]);
@@ -60,8 +62,8 @@ template <int D> XPU_DEVICE void keep8(const KeepArgs &a, uint32_t per_block) {
   const uint32_t in_page = slot_of(lane * kBlock) / kBlock;
 
   const bool apart = per_block != 1u && count <= 16u;  // the wavefronts work on parts of their own
-  for (uint32_t step = 0; step < (apart ? 1u : per_block); ++step) {
-    const uint32_t part = group * per_block + (apart ? wave : step), row = apart ? 0u : wave * 16u;
+  for (uint32_t step = apart ? wave : 0u; step < per_block; step += apart ? 4u : 1u) {
+    const uint32_t part = group * per_block + step, row = apart ? 0u : wave * 16u;
     if (part >= parts) break;
     const bool lead = apart || wave == 0;  // has the part's scales and earlier rows
     const uint32_t head = part / 2u % a.pool.kv_heads, layer = part / 2u / a.pool.kv_heads;

@@ -95,7 +95,7 @@ struct KeepArgs {
 
 struct Keep8Args {
   KeepArgs keep;
-  uint32_t per_block;  // parts (layer, kv head, K or V) that a block takes: 1 or 4
+  uint32_t per_block;  // parts (layer, kv head, K or V) that a block takes: 1, or a multiple of 4
 };
 
 // The rotation of rows on their way (half = rotated dims / 2; 0: none).
