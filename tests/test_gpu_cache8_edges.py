@@ -1,0 +1,76 @@
+"""The 8-bit paged cache on gfx950 where rows are left out: rows without angles,
+without a place, of no sequence."""
+import numpy as np
+import pytest
+
+import xpu_playground_amd as xpu
+from cache8_util import Pool8
+from cache_util import Buffers, codes, normal, u32
+from test_gpu_cache8 import TYPES, f32
+
+pytestmark = pytest.mark.gpu
+
+
+def written(pool, layer, table, context, rows, skip=()):
+    """What an append makes of rows whose `skip` are written to neither pool."""
+    for n, x in rows.items():
+        held = pool.codes, pool.scales
+        pool.codes, pool.scales = {"k": held[0][n]}, {"k": held[1][n]}
+        pool.append(layer, table, context, {"k": x}, skip)
+        pool.codes, pool.scales = held
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,kv,page", [(64, 2, 16), (128, 1, 32)])
+@pytest.mark.parametrize("adjacent", [False, True])
+def test_rows_without_angles_are_not_written(rt, dtype, d, kv, page, adjacent):
+    """Neither K nor V, nor do they take part in their blocks' scales, however
+    large: first, in between, last and all of a block's rows; the rows before the
+    batch's in the block stay as they are. cos 1 and sin 0 turn nothing, so K is
+    byte for byte too."""
+    with Buffers(rt) as b:
+        pool = Pool8(rt, b, 6, kv, d, page, 1, dtype)
+        tables, n = u32([[4, 1, 3, 2]]), 37
+        k, v = normal((n, kv * d), 5, dtype), normal((n, kv * d), 6, dtype)
+        fk, fv = (f32(x, dtype).reshape(n, kv, d) for x in (k, v))
+        before = normal((3, kv * d), 7, dtype)
+        fb = f32(before, dtype).reshape(3, kv, d)
+        rt.cache8_append(pool.cache, xpu.Batch(1, 3, 4, b.up(tables), b.up(u32([0, 3])), b.up(u32([0]))), 0, b.up(before), b.up(before))
+        pool.append(0, tables[0], 0, {"k": fb, "v": fb})
+        pool.verify()
+        cos, sin = np.ones((3, d // 2), np.float32), np.zeros((3, d // 2), np.float32)
+        skip = [0, 5, 12] + list(range(13, 29)) + [36]  # positions 3, 8, 15; block 1 (16 .. 31); 39
+        for i in skip:
+            k[i] = v[i] = codes(np.full(kv * d, 3e4), dtype)
+        at = u32([9 if i in skip else i % 3 for i in range(n)])
+        at[36] = 0xFFFFFFFF
+        rotary = xpu.Rotary(3, d, b.up(cos), b.up(sin), xpu.ADJACENT if adjacent else xpu.HALVES, b.up(at))
+        batch = xpu.Batch(1, n, 4, b.up(tables), b.up(u32([0, n])), b.up(u32([3])))
+        print(f"append8 without angles d {d} kv {kv} page {page} dtype {dtype}", flush=True)
+        rt.cache8_append(pool.cache, batch, 0, b.up(k), b.up(v), rotary)
+        written(pool, 0, tables[0], 3, {"k": fk, "v": fv}, skip)
+        pool.verify(status=1)
+
+
+def test_rows_without_a_place_or_a_position(rt):
+    """A page past the pool, positions past the table, starts that do not fit, and
+    positions past the tables of angles in a block that they begin."""
+    with Buffers(rt) as b:
+        pool = Pool8(rt, b, 5, 2, 64, 16, 1)
+        k, v = normal((12, 128), 5, pool.dtype), normal((12, 128), 6, pool.dtype)
+        fk, fv = f32(k, pool.dtype).reshape(12, 2, 64), f32(v, pool.dtype).reshape(12, 2, 64)
+        tables = u32([[0, 5], [1, 2]])
+        dk, dv, dt = b.up(k), b.up(v), b.up(tables)
+        rt.cache8_append(pool.cache, xpu.Batch(2, 12, 2, dt, b.up(u32([0, 4, 8])), b.up(u32([14, 30]))), 0, dk, dv)
+        written(pool, 0, tables[0], 14, {"k": fk[:2], "v": fv[:2]})
+        written(pool, 0, tables[1], 30, {"k": fk[4:6], "v": fv[4:6]})
+        pool.verify(status=1)
+        for starts, context in ([0, 0xFFFFFFF0, 8], [0, 0]), ([6, 3, 1], [0, 0]), ([0, 0, 4], [0, 0xFFFFFFFE]):
+            rt.cache8_append(pool.cache, xpu.Batch(2, 12, 2, dt, b.up(u32(starts)), b.up(u32(context))), 0, dk, dv)
+        pool.verify(status=1)
+        cos, sin = np.ones((3, 32), np.float32), np.zeros((3, 32), np.float32)
+        rotary = xpu.Rotary(3, 64, b.up(cos), b.up(sin), eps=0.0)
+        rt.copy_to(pool.status, u32([0]))
+        rt.cache8_append(pool.cache, xpu.Batch(1, 5, 1, b.up(u32([[3]])), b.up(u32([0, 5])), b.up(u32([0]))), 0, dk, dv, rotary)
+        written(pool, 0, u32([3]), 0, {"k": fk[:5], "v": fv[:5]}, skip=(3, 4))
+        pool.verify(status=1)

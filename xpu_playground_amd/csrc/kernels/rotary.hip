@@ -309,14 +309,14 @@ template <int DT, int D> XPU_DEVICE void append_block(const RotateArgs &a, const
     const uint32_t j = l * kPer + lane / kGroup, row = row0 + min(j, count - 1u);
     unpack8<DT>(*reinterpret_cast<const u32x4 *>(from + row * stride), x[l]);
     real[l] = j < count;
-    if (!is_v && (a.rot.half || a.rot.k_gain)) {
+    if (a.rot.half) {  // (a row without angles is not written, neither K nor V)
       const uint64_t at = a.rot.at ? a.rot.at[row] : start + held + j;
       const uint32_t turned = at < 0xffffffffull ? static_cast<uint32_t>(at) : 0xffffffffu;
-      if (a.rot.half && turned >= a.rot.positions) {
+      if (turned >= a.rot.positions) {
         odd |= real[l];
         real[l] = false;
       }
-      turn<DT, D>(x[l], a.rot, angles_of<D>(a.rot, turned), a.rot.k_gain);
+      if (!is_v) turn<DT, D>(x[l], a.rot, angles_of<D>(a.rot, turned), a.rot.k_gain);
     }
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
