@@ -697,7 +697,8 @@ template <int DT> XPU_DEVICE void list(const SampleArgs &a) {
     if (bins.counts(n.k)) {
       const uint32_t b = bins.find(true, n.k);
       ranges[2] = Range(bins, b, b);
-      lo = bins.weight_before(b) + 1u;
+      // (the bin's first tokens, or all of it, may round to nothing; the first bin does not)
+      lo = b ? bins.weight_before(b) : 1u;
       hi = bins.weight_to(b);
     }
     if (n.p < 1.0f) {
