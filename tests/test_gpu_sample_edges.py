@@ -1,5 +1,6 @@
 """xpu_sample on gfx950 where its launches meet: bins whose weight rounds to
-nothing."""
+nothing, temperatures at which neighbouring floats are further apart than the
+histogram is long."""
 import numpy as np
 import pytest
 
@@ -8,6 +9,7 @@ from cache_util import Buffers
 from test_gpu_sample import Rows
 
 pytestmark = pytest.mark.gpu
+NEAR_ONE = np.float32(1 - 2.0 ** -24)
 
 
 def call(rt, r):
@@ -37,3 +39,18 @@ def test_a_last_token_that_weighs_nothing(rt, vocab, p):
     share = np.exp(np.float32([0.0, -0.5])) / 2  # of a sum of 2, to 2^-44
     i = [at[0], at[256]].index(token[0])
     assert abs(probability[0] - share[i]) <= 2.0 ** -22 * share[i]
+
+
+@pytest.mark.parametrize("top,t", [(2.0 ** 24, 0.0185), (30.0, 3.5e-8), (-1e6, 1.2e-3), (1e30, 1.36e21)])
+@pytest.mark.parametrize("vocab", [500, 20000])
+def test_neighbouring_floats_far_apart(rt, top, t, vocab):
+    """The next float below the largest logit is 78 powers of two less in weight:
+    nothing, of however many tokens."""
+    top = np.float32(top)
+    x = np.full((3, vocab), np.nextafter(top, np.float32(-np.inf)))
+    x[0, 77] = x[1, vocab - 1] = x[2, 0] = x[2, 300] = top
+    gap = (float(top) - float(x[0, 0])) / t * 1.4427 * 32
+    assert 2048 < gap < 3198  # in bins: past the slots, nearer to the last bin than the largest is
+    for numbers in (dict(), dict(k=300), dict(p=0.99999), dict(k=40)):
+        got = Rows(x, xpu.FP32, t=t, u=NEAR_ONE, **numbers).verify(rt)
+        assert list(got) == [77, vocab - 1, 300]

@@ -226,10 +226,13 @@ struct Weights {
     const double y = __builtin_fma(q, powers[static_cast<uint32_t>(bin) % kSteps], lift);
     return {bin, __builtin_bit_cast(uint64_t, y) & 0xfffffffffffffull};
   }
-  // A logit below all of bins from `bin` on; those from it on have bins of 32 bits.
+  // A logit below all of bins from `bin` on; those from it on have bins of 32
+  // bits, and are 64 bins below `bin` at most: the first float from there up, as
+  // the nearest may be any number of bins further down.
   XPU_DEVICE float below(int32_t bin) const {
     const double d = (static_cast<double>(bin) - 64.0) * width + base;
-    return static_cast<float>(__builtin_fmax(d, -0x1.fffffep127));
+    const float f = static_cast<float>(__builtin_fmax(d, -0x1.fffffep127));
+    return f < d ? of_ordered(ordered(f) + 1u) : f;
   }
 };
 // Units of n as units of a larger n.
