@@ -65,9 +65,9 @@ int xpu_tree_attention8_workspace(const xpu_runtime *rt, const xpu_cache8 *cache
 
 /* xpu_cache_keep in 8 bits: the same arguments. A block that kept rows reach
  * gets the largest scale of its own and of the blocks that they come from; the
- * codes of the rows that come, and of the sequence's rows before them, are
- * rounded to it where it is larger than theirs. The positions behind the kept
- * ones hold nothing of use. */
+ * codes of the rows that come, of the sequence's rows before them, and of rows
+ * left alone as their node does not exist, are rounded to it where it is larger
+ * than theirs. The positions behind the kept ones hold nothing of use. */
 int xpu_cache8_keep(xpu_runtime *rt, const xpu_cache8 *cache, const xpu_batch *batch, const uint32_t *kept,
                     const uint32_t *counts, uint32_t *new_context);
 

@@ -1,5 +1,5 @@
 """The 8-bit paged cache on gfx950 where rows are left out: rows without angles,
-without a place, of no sequence."""
+without a place, of no sequence; kept nodes that do not exist."""
 import numpy as np
 import pytest
 
@@ -73,4 +73,52 @@ def test_rows_without_a_place_or_a_position(rt):
         rt.copy_to(pool.status, u32([0]))
         rt.cache8_append(pool.cache, xpu.Batch(1, 5, 1, b.up(u32([[3]])), b.up(u32([0, 5])), b.up(u32([0]))), 0, dk, dv, rotary)
         written(pool, 0, u32([3]), 0, {"k": fk[:5], "v": fv[:5]}, skip=(3, 4))
+        pool.verify(status=1)
+
+
+@pytest.mark.parametrize("d,kv,layers,seqs", [(64, 1, 1, 1), (128, 2, 1, 3), (64, 2, 3, 2), (64, 8, 4, 40)])
+@pytest.mark.parametrize("more", [0, 20])
+def test_a_kept_node_that_does_not_exist(rt, d, kv, layers, seqs, more):
+    """The place it would have gone to holds the value that it held, also where
+    the block's scale grows by a row from another block. more: nodes kept
+    besides, for the form that takes more than 16. 40 sequences: more parts than
+    blocks at once."""
+    rng = np.random.RandomState(1)
+    context, n = 3, 40
+    with Buffers(rt) as b:
+        pool = Pool8(rt, b, 3 * seqs, kv, d, 16, layers)
+        tables = u32(rng.permutation(3 * seqs).reshape(seqs, 3))
+        for name in "kv":  # a block's scale is larger than the one's before it
+            for t in tables:
+                pool.scales[name][:, t] = np.array([110, 112, 115])[None, :, None, None]
+            rt.copy_to(pool.ptr[name], pool.raw(name))
+        kept = [0xFFFFFFFF, 17, 64, 2, n] + list(range(more))  # 17: position 20, of the second block
+        flat = u32(np.tile(kept + [0] * (n - len(kept)), seqs))
+        batch = xpu.Batch(seqs, n * seqs, 3, b.up(tables), b.up(u32(np.arange(seqs + 1) * n)), b.up(u32([context] * seqs)))
+        print(f"keep8 d {d} kv {kv} layers {layers} seqs {seqs} more {more}", flush=True)
+        rt.cache8_keep(pool.cache, batch, b.up(flat), b.up(u32([len(kept)] * seqs)))
+        for t in tables:
+            # the nodes that do not exist stay where they are
+            pool.keep(t, context, [i if i < n else j for j, i in enumerate(kept)], n)
+        pool.verify(status=1)
+
+
+def test_a_kept_node_whose_page_does_not_exist(rt):
+    """The same where a node's own page is missing; a place whose page is missing
+    gets nothing."""
+    with Buffers(rt) as b:
+        pool = Pool8(rt, b, 4, 2, 64, 16, 2)
+        tables = u32([[0, 9, 2], [1, 3, 9]])
+        for name in "kv":
+            for p, s in ((0, 110), (2, 118), (1, 111), (3, 114)):
+                pool.scales[name][:, p] = s
+            rt.copy_to(pool.ptr[name], pool.raw(name))
+        # sequence 0: node 13 (position 16) is on the missing page, node 30 (position 33) raises page 0's scale.
+        # sequence 1: node 31 (position 34) is on the missing page
+        kept = [[13, 30, 1] + list(range(3, 20)), [31, 14, 15, 2]]
+        flat = u32(sum((ids + [0] * (40 - len(ids)) for ids in kept), []))
+        batch = xpu.Batch(2, 80, 3, b.up(tables), b.up(u32([0, 40, 80])), b.up(u32([3, 3])))
+        rt.cache8_keep(pool.cache, batch, b.up(flat), b.up(u32([len(ids) for ids in kept])))
+        for t, ids in zip(tables, kept):
+            pool.keep(t, 3, [i if int(t[(3 + i) // 16]) < 4 else j for j, i in enumerate(ids)], 40)
         pool.verify(status=1)

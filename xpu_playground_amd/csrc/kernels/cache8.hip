@@ -46,15 +46,19 @@ template <int D> XPU_DEVICE void keep8(const KeepArgs &a, uint32_t per_block) {
   };
   auto slot_of = [&](uint32_t at) { return (within + at) & (a.pool.page_size - 1u); };
 
-  // where each node goes: lane j is kept node j
-  const uint32_t node = a.kept[lo + (lane < count ? lane : 0u)];
-  const bool exists = node < hi - lo && node < 64u;
-  const uint64_t from_page = page_of(in + (exists ? node : 0u)), to_page = page_of(in + lane);
-  const bool real = lane < count, fine = real && exists && from_page != kNowhere && to_page != kNowhere;
-  const uint32_t from_block = (in + (exists ? node : 0u)) / kBlock, to_block = (in + lane) / kBlock;
-  const uint64_t from = from_page + static_cast<uint64_t>(slot_of(in + (exists ? node : 0u))) * D;
+  // where each node goes: lane j is kept node j. A place whose node does not exist
+  // holds what it held: its own node, which is rescaled with its block.
+  const uint32_t asked = a.kept[lo + (lane < count ? lane : 0u)];
+  const bool exists = asked < hi - lo && asked < 64u;
+  const uint64_t asked_page = page_of(in + (exists ? asked : 0u)), to_page = page_of(in + lane);
+  const bool known = exists && asked_page != kNowhere;
+  const uint32_t node = known ? asked : lane;
+  const uint64_t from_page = known ? asked_page : to_page;
+  const bool real = lane < count, fine = real && to_page != kNowhere;
+  const uint32_t from_block = (in + node) / kBlock, to_block = (in + lane) / kBlock;
+  const uint64_t from = from_page + static_cast<uint64_t>(slot_of(in + node)) * D;
   const uint64_t to = to_page + static_cast<uint64_t>(slot_of(in + lane)) * D;
-  if (__builtin_amdgcn_ballot_w64(real && !fine)) report(a.pool);
+  if (__builtin_amdgcn_ballot_w64(real && !(known && fine))) report(a.pool);
   // the blocks, lanes 0 .. 4
   const uint32_t reach = in + (hi - lo < 64u ? hi - lo : 64u);  // places with nodes
   const uint64_t block_page = page_of(min(lane, 4u) * kBlock), page0 = page_of(0);
