@@ -1,10 +1,10 @@
 """The 8-bit paged cache on gfx950 where rows are left out: rows without angles,
-without a place, of no sequence; kept nodes that do not exist."""
+without a place, that an earlier sequence claims; kept nodes that do not exist."""
 import numpy as np
 import pytest
 
 import xpu_playground_amd as xpu
-from cache8_util import Pool8
+from cache8_util import BLOCK, Pool8, rescaled, scale_byte, values8
 from cache_util import Buffers, codes, normal, u32
 from test_gpu_cache8 import TYPES, f32
 
@@ -122,3 +122,56 @@ def test_a_kept_node_whose_page_does_not_exist(rt):
         for t, ids in zip(tables, kept):
             pool.keep(t, 3, [i if int(t[(3 + i) // 16]) < 4 else j for j, i in enumerate(ids)], 40)
         pool.verify(status=1)
+
+
+@pytest.mark.parametrize("starts", [[0, 5, 3, 8], [0, 20, 3, 24]])
+def test_rows_that_an_earlier_sequence_claims(rt, starts):
+    """The last sequence begins with rows of the first; those behind them are its
+    own alone, in a block of which it has no earlier rows: what the block held
+    before is not in their scale."""
+    with Buffers(rt) as b:
+        pool = Pool8(rt, b, 8, 2, 64, 16, 1)
+        for n in "kv":
+            pool.scales[n][:] = 200
+            rt.copy_to(pool.ptr[n], pool.raw(n))
+        n, first = starts[3], starts[1]
+        k, v = normal((n, 128), 5, pool.dtype), normal((n, 128), 6, pool.dtype)
+        tables = u32([[0, 1], [2, 3], [4, 5]])
+        batch = xpu.Batch(3, n, 2, b.up(tables), b.up(u32(starts)), b.up(u32([0, 0, 0])))
+        rt.cache8_append(pool.cache, batch, 0, b.up(k), b.up(v))
+        rt.synchronize()
+        for name, x in (("k", k), ("v", v)):
+            got, scales = pool.parts(pool.load(name))
+            rows = f32(x, pool.dtype).reshape(n, 2, 64)
+            for i in range(first, n):
+                p, slot = pool.place(tables[2], i - starts[2])
+                block = [j for j in range(starts[2], n) if (j - starts[2]) // BLOCK == (i - starts[2]) // BLOCK]
+                for h in range(2):
+                    scale = int(scales[0, p, h, 0])
+                    assert scale <= scale_byte(np.abs(rows[block, h]).max())  # with or without the claimed rows
+                    value = np.ldexp(values8(got[0, p, h, slot]), scale - 127)
+                    assert (np.abs(value - rows[i, h]) <= 2.0 ** -4 * np.abs(rows[i, h]) + 2.0 ** (scale - 127 - 10)).all()
+
+
+def test_rows_behind_claimed_ones_in_a_block_with_earlier_rows(rt):
+    """Here the last sequence has 5 positions in the block, which are rescaled
+    where its own row raises the scale."""
+    with Buffers(rt) as b:
+        pool = Pool8(rt, b, 8, 1, 64, 16, 1)
+        tables = u32([[0], [1], [2]])
+        before = normal((5, 64), 7, pool.dtype)
+        rt.cache8_append(pool.cache, xpu.Batch(1, 5, 1, b.up(tables[2:]), b.up(u32([0, 5])), b.up(u32([0]))), 0, b.up(before), b.up(before))
+        fb = f32(before, pool.dtype).reshape(5, 1, 64)
+        pool.append(0, tables[2], 0, {"k": fb, "v": fb})
+        rows = normal((6, 64), 8, pool.dtype, 40.0)
+        batch = xpu.Batch(3, 6, 1, b.up(tables), b.up(u32([0, 5, 3, 6])), b.up(u32([0, 0, 5])))
+        rt.cache8_append(pool.cache, batch, 0, b.up(rows), b.up(rows))
+        rt.synchronize()
+        got, scales = pool.parts(pool.load("k"))
+        scale, old = int(scales[0, 2, 0, 0]), int(pool.scales["k"][0, 2, 0, 0])
+        assert scale > old
+        a, c = got[0, 2, 0, :5].copy(), rescaled(pool.codes["k"][0, 2, 0, :5], old - scale)
+        assert np.array_equal(values8(a), values8(c))
+        x = f32(rows, pool.dtype)[5]
+        value = np.ldexp(values8(got[0, 2, 0, 7]), scale - 127)
+        assert (np.abs(value - x) <= 2.0 ** -4 * np.abs(x) + 2.0 ** (scale - 127 - 10)).all()

@@ -249,6 +249,7 @@ struct BlockAt {
   uint32_t block;     // of the sequence's reached ones
   uint32_t first, n;  // the sequence's rows
   uint64_t context;   // positions before them
+  uint32_t claimed;   // of these positions, the last ones that are an earlier sequence's rows
 };
 XPU_DEVICE BlockAt block_at(const BatchArgs &b, uint32_t item) {
   uint32_t before = 0, taken = 0;  // blocks and rows of the sequences before
@@ -269,23 +270,24 @@ XPU_DEVICE BlockAt block_at(const BatchArgs &b, uint32_t item) {
       const uint32_t l = __builtin_ctzll(hit);
       auto of = [&](uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(v, l)); };
       return {static_cast<int32_t>(at + l), item - of(upto - count), of(first), of(n),
-              static_cast<uint64_t>(of(c)) + of(first - lo)};
+              static_cast<uint64_t>(of(c)) + of(first - lo), of(first - lo)};
     }
     before = __builtin_amdgcn_readlane(upto, 63);
     taken = __builtin_amdgcn_readlane(most, 63);
   }
-  return {-1, 0, 0, 0, 0};
+  return {-1, 0, 0, 0, 0, 0};
 }
 
 // 8 bits: the rows of one block of one kv head, K or V, by a wavefront.
 template <int DT, int D> XPU_DEVICE void append_block(const RotateArgs &a, const BlockAt &b, uint32_t head, bool is_v) {
   constexpr uint32_t kGroup = D / 8, kPer = 64 / kGroup, kLoads = kBlock / kPer;
   const uint32_t lane = lane_id(), dim = lane % kGroup * 8u;
-  const uint32_t in = static_cast<uint32_t>(b.context) & (kBlock - 1u);  // earlier rows of the first block
+  const uint32_t in = static_cast<uint32_t>(b.context) & (kBlock - 1u);  // positions of the first block before the rows
   const uint64_t start = b.context - in + static_cast<uint64_t>(b.block) * kBlock;
-  const uint32_t held = b.block ? 0u : in;
-  const uint32_t done = b.block ? b.block * kBlock - in : 0u;  // rows in earlier blocks
-  const uint32_t count = min(b.n - done, kBlock - held), row0 = b.first + done;
+  const uint32_t before = b.block ? 0u : in;
+  const uint32_t held = before > b.claimed ? before - b.claimed : 0u;  // rows that the sequence has there
+  const uint32_t done = b.block ? b.block * kBlock - in : 0u;          // rows in earlier blocks
+  const uint32_t count = min(b.n - done, kBlock - before), row0 = b.first + done;
   const uint64_t place = element_of(a.pool, a.batch.tables + static_cast<uint64_t>(b.seq) * a.batch.table_pitch,
                                     a.batch.table_pitch, start, D);
   if (place == kNowhere) {
@@ -310,7 +312,7 @@ template <int DT, int D> XPU_DEVICE void append_block(const RotateArgs &a, const
     unpack8<DT>(*reinterpret_cast<const u32x4 *>(from + row * stride), x[l]);
     real[l] = j < count;
     if (a.rot.half) {  // (a row without angles is not written, neither K nor V)
-      const uint64_t at = a.rot.at ? a.rot.at[row] : start + held + j;
+      const uint64_t at = a.rot.at ? a.rot.at[row] : start + before + j;
       const uint32_t turned = at < 0xffffffffull ? static_cast<uint32_t>(at) : 0xffffffffu;
       if (turned >= a.rot.positions) {
         odd |= real[l];
@@ -342,7 +344,7 @@ template <int DT, int D> XPU_DEVICE void append_block(const RotateArgs &a, const
   for (uint32_t l = 0; l < kLoads; ++l) {
     const uint32_t j = l * kPer + lane / kGroup;
     const u32x2 c = codes8(x[l], now);
-    if (real[l]) *reinterpret_cast<u32x2 *>(codes + (held + j) * D) = c;
+    if (real[l]) *reinterpret_cast<u32x2 *>(codes + (before + j) * D) = c;
   }
   if (lane == 0) *scale = static_cast<uint8_t>(now);
 }
