@@ -148,8 +148,9 @@ int xpu_qwen3_set_attention_split(xpu_qwen3 *eng, uint32_t min_context);
  * continuation with the same seed draws what one call would have. Temperature 0
  * (the default) takes the argmax and ignores the others but for their ranges;
  * XPU_ERR_INVALID for a temperature that is negative or not finite, a negative
- * top_p, a min_p outside [0, 1], NaN, or a vocabulary above 2^20. The first call
- * with a temperature allocates. The reference is greedy only. */
+ * top_p, a min_p outside [0, 1], NaN, or a vocabulary above 2^20. A non-finite
+ * logit, -infinity too, fails as without sampling (XPU_ERR_VERIFY), in all modes.
+ * The first call with a temperature allocates. The reference is greedy only. */
 int xpu_qwen3_set_sampling(xpu_qwen3 *eng, float temperature, uint32_t top_k, float top_p, float min_p, uint64_t seed);
 
 /* One forward step at `position` for input `token`; *next = greedy token

@@ -1162,11 +1162,11 @@ extern "C" __global__ __launch_bounds__(1024) void xpu_q3_argmax_finish(
   }
 }
 
-// A drawn token gen[index] (xpu_sample wrote it there over the argmax) as the
-// next step's input, behind xpu_q3_argmax_finish.
-extern "C" __global__ __launch_bounds__(64) void xpu_q3_take_token(uint32_t *state, const uint32_t *__restrict__ gen,
-                                                                    uint32_t index) {
-  if (threadIdx.x == 0) state[1] = state[2] = gen[index];
+// A drawn token in place of the argmax, as gen[index] and the next step's input,
+// behind xpu_q3_argmax_finish; not where that marked a non-finite logit.
+extern "C" __global__ __launch_bounds__(64) void xpu_q3_take_token(uint32_t *state, uint32_t *__restrict__ gen,
+                                                                    uint32_t index, const uint32_t *__restrict__ drawn) {
+  if (threadIdx.x == 0 && state[2] != 0xffffffffu) gen[index] = state[1] = state[2] = *drawn;
 }
 
 // ------------------------------------------------------------ batched prefill

@@ -189,9 +189,11 @@ struct xpu_qwen3 {
     uint32_t block = 0;
   } pf_qkv_m, pf_o_m, pf_gu_m, pf_down_m;
   // sampling in generate (xpu_qwen3_set_sampling): one block, allocated by
-  // the first call; draws[p] is the random number behind position p
+  // the first call: the four numbers, the token drawn, the random number behind
+  // each position, the workspace
   bool sampling = false;
   void *sample_block = nullptr;
+  uint32_t *drawn = nullptr;
   xpu_sampling sample{};
   void *sample_workspace = nullptr;
   uint64_t sample_bytes = 0;
@@ -1316,6 +1318,7 @@ extern "C" int xpu_qwen3_set_sampling(xpu_qwen3 *eng, float temperature, uint32_
     s.top_p = at + 2;
     s.min_p = at + 3;
     s.random = at + 64;
+    e.drawn = static_cast<uint32_t *>(e.sample_block) + 4;
     e.sample = s;
     e.sample_workspace = static_cast<uint8_t *>(e.sample_block) + 256 + draws;
     e.sample_bytes = bytes;
@@ -1326,19 +1329,20 @@ extern "C" int xpu_qwen3_set_sampling(xpu_qwen3 *eng, float temperature, uint32_
 
 namespace {
 
-// With sampling: draws generated token `index`, the one behind `position`, of
-// the step's logits into gen.
-int draw_token(xpu_qwen3 &e, uint32_t position, uint32_t index) {
+// With sampling: draws the token behind `position` of the step's logits, into
+// `drawn`.
+int draw_token(xpu_qwen3 &e, uint32_t position) {
   xpu_sampling s = e.sample;
   s.random += position;
-  return xpu_sample(e.rt, &s, e.logits, e.gen + index, nullptr, e.sample_workspace, e.sample_bytes);
+  return xpu_sample(e.rt, &s, e.logits, e.drawn, nullptr, e.sample_workspace, e.sample_bytes);
 }
 
-// The same behind a fused step, whose argmax it replaces.
+// The same behind a fused step, in place of its argmax as generated token `index`
+// (unless it marked a non-finite logit, as all modes refuse such a step).
 int replace_token(xpu_qwen3 &e, uint32_t position, uint32_t index) {
   if (!e.sampling) return XPU_OK;
-  const int rc = draw_token(e, position, index);
-  return rc ? rc : launch(e, e.take_l, 64, {{8, &e.state}, {8, &e.gen}, {4, &index}});
+  const int rc = draw_token(e, position);
+  return rc ? rc : launch(e, e.take_l, 64, {{8, &e.state}, {8, &e.gen}, {4, &index}, {8, &e.drawn}});
 }
 
 }  // namespace
@@ -1420,8 +1424,8 @@ extern "C" int xpu_qwen3_generate(xpu_qwen3 *eng, const uint32_t *prompt, uint32
     uint32_t next = 0;
     auto draw = [&](uint32_t index) {
       if (!eng->sampling) return XPU_OK;
-      int failed = draw_token(*eng, n_prompt - 1 + index, index);
-      if (!failed) failed = xpu_rt_copy_from_device(eng->rt, &next, eng->gen + index, 4);
+      int failed = draw_token(*eng, n_prompt - 1 + index);
+      if (!failed) failed = xpu_rt_copy_from_device(eng->rt, &next, eng->drawn, 4);
       return failed || next != XPU_SAMPLE_NONE
                  ? failed
                  : set_error(XPU_ERR_VERIFY, "model produced a NaN or infinity in vocabulary logits");
