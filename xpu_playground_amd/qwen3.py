@@ -8,11 +8,12 @@ path.
 from __future__ import annotations
 
 import ctypes
+import struct
 from ctypes import c_double, c_uint32, c_void_p
 
 import numpy as np
 
-from . import Qwen3Config, Runtime, check, library
+from . import Qwen3Config, Runtime, _fit, check, library
 
 GRAPH, EAGER, REFERENCE = 0, 1, 2
 EOS_TOKENS = (151645, 151643)  # qwen3/model.hpp:19-20
@@ -128,6 +129,7 @@ class Engine:
                      seed: int = 0) -> None:
         """Draw the tokens of generate (xpu_sample with random numbers hashed
         from seed and position); temperature 0 takes the argmax again."""
+        _fit("set_sampling", struct.Struct("=IQ"), top_k, seed)
         check(self.lib.xpu_qwen3_set_sampling(self.handle, temperature, top_k, top_p, min_p, seed))
 
     def decode(self, token: int, position: int) -> int:
