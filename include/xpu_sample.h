@@ -32,9 +32,11 @@ extern "C" {
  * times the kept ones' sum. Temperature 0 keeps the first token alone. A logit
  * of -infinity is never drawn. The numbers of the rows are on the device, one
  * per row; NULL is temperature 1, or no filter. Weights are formed in 64 bits
- * and summed as integers, off by half of 2^-41 of the largest weight per token
- * at most (2^-44 up to 2^17 tokens) in any order, so a row's token does not
- * depend on the rows beside it; a weight below 2^-47 of the largest is 0. */
+ * and summed as integers, off by 2^-41 of the largest weight per token at most
+ * (2^-44 up to 2^17 tokens); weights below 2^-47 of the largest may count as 0. A
+ * row's token does not depend on what the rows beside it hold. How a row is summed
+ * goes by the numbers of rows and tokens, so with other numbers of rows it may be
+ * drawn otherwise where random times the sum is that near to a token's border. */
 typedef struct {
   int32_t dtype;            /* of the logits: XPU_DTYPE_BF16, _FP16 or _FP32 */
   uint32_t rows;

@@ -18,7 +18,7 @@
 // largest's n. So sums do not depend on their order, no
 // bin depends on the largest logit, and one pass over the row gives both. A sum
 // is off by half a unit per token and per bin (fine + log2 of the tokens is 61
-// at most), and weights below 2^-47 of the largest count as nothing.
+// at most), and weights below 2^-47 of the largest may count as nothing.
 //
 // Three launches. xpu_sample_look, several blocks to a row: the histogram of
 // the weights. xpu_sample_list, the same blocks: which bins the k-th token, the
