@@ -8,13 +8,16 @@
  *
  * A position's K and V are codes of 8 bits (e4m3: 4 significant bits, largest
  * 448) times a scale that 16 positions of a kv head share, a power of two. A
- * block of 16 positions gets the smallest scale with which all of its rows'
- * finite values are at most 448 codes (2^-100 at least). Rows that come later
- * to a block of which the sequence has earlier rows never lower it; where they
- * raise it, the codes of the earlier rows are rounded once more to the new
- * one. A value is off by half a code's step, 2^-4 of itself or, if small, 2^-17
- * of the block's largest. Infinities and NaN are stored as NaN; a value whose
- * code stands for more than the largest number of `dtype` reads as infinite.
+ * block of 16 positions gets the smallest scale with which all finite values of
+ * the rows that come to it in one call are at most 448 codes (2^-100 at least),
+ * or keeps its scale where it holds earlier positions of the sequence and that is
+ * larger: a scale never falls while they stay. Where it grows, their codes are
+ * rounded once more to the new one. So a block's scale is that of the largest row
+ * that came to it since its first, rejected rows included, or that came to a block
+ * of which xpu_cache8_keep moved a row here; that row's largest value is above 224
+ * scales (or the scale 2^-100). A value is off by 2^-4 of itself and 2^-9 of its
+ * block's scale at most. Infinities and NaN are stored as NaN; a value whose code
+ * stands for more than the largest number of `dtype` reads as infinite.
  */
 #ifndef XPU_CACHE8_H
 #define XPU_CACHE8_H

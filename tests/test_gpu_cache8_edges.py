@@ -1,11 +1,12 @@
 """The 8-bit paged cache on gfx950 where rows are left out: rows without angles,
-without a place, that an earlier sequence claims; kept nodes that do not exist."""
+without a place, that an earlier sequence claims; kept nodes that do not exist;
+and how far rows are off that share a block with rejected and moved ones."""
 import numpy as np
 import pytest
 
 import xpu_playground_amd as xpu
 from cache8_util import BLOCK, Pool8, rescaled, scale_byte, values8
-from cache_util import Buffers, codes, normal, u32
+from cache_util import Buffers, codes, normal, u32, values
 from test_gpu_cache8 import TYPES, f32
 
 pytestmark = pytest.mark.gpu
@@ -175,3 +176,54 @@ def test_rows_behind_claimed_ones_in_a_block_with_earlier_rows(rt):
         x = f32(rows, pool.dtype)[5]
         value = np.ldexp(values8(got[0, 2, 0, 7]), scale - 127)
         assert (np.abs(value - x) <= 2.0 ** -4 * np.abs(x) + 2.0 ** (scale - 127 - 10)).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_beside_rejected_and_moved_ones(rt, dtype):
+    """Rows are off by 2^-4 of themselves and 2^-9 of their block's scale at most:
+    the first rounding is off by 2^-4 of the value or, below the normal codes, by
+    2^-10 of the scale then; as a scale grows, codes that leave the normal ones are
+    rounded again, by 2^-10 of the scale it gets; scales grow by factors of two and
+    more, so these add up to less than 2^-9 of the last. The last is what the
+    largest row needed that came to the block or to the block of a row moved here,
+    rejected ones included."""
+    rng = np.random.RandomState(2)
+    with Buffers(rt) as b:
+        pool = Pool8(rt, b, 4, 1, 64, 16, 1, dtype)
+        tables = u32([[2, 0, 1]])
+        dt, up = b.up(tables), lambda *x: b.up(u32(x))
+        held = {}  # position -> row
+
+        def append(at, size):
+            row = codes(rng.randn(len(size), 64) * np.array(size, float)[:, None] * 2.0 ** rng.randint(-14, 1, (len(size), 64)), dtype)
+            rt.cache8_append(pool.cache, xpu.Batch(1, len(size), 3, dt, up(0, len(size)), up(at)), 0, b.up(row), b.up(row))
+            held.update((at + i, x) for i, x in enumerate(values(row, dtype)))
+            return values(row, dtype)
+
+        def far(n, tops):
+            rt.synchronize()
+            for name in "kv":
+                got, scales = pool.parts(pool.load(name))
+                for pos in range(n):
+                    p, slot = pool.place(tables[0], pos)
+                    scale = 2.0 ** (int(scales[0, p, 0, 0]) - 127)
+                    assert scale == 2.0 ** (scale_byte(tops[pos // BLOCK]) - 127)
+                    value = np.ldexp(values8(got[0, p, 0, slot]), int(scales[0, p, 0, 0]) - 127)
+                    x = held[pos]
+                    assert (np.abs(value - x) <= 2.0 ** -4 * np.abs(x) + 2.0 ** -9 * scale).all(), (name, pos)
+
+        tops = [np.abs(append(0, [1.0] * 5)).max()]
+        far(5, tops)
+        for size in (4.0, 9.0, 64.0):  # drafts that are rejected
+            tops[0] = max(tops[0], np.abs(append(5, [0.5, size, 1.0])).max())
+            far(5, tops)
+        tops[0] = max(tops[0], np.abs(append(5, [1.0])).max())
+        far(6, tops)
+        # a draft into the next two blocks, of which the small row at position 20 is kept: it
+        # brings the scale of its block, which a large row beside it has set
+        rows = append(6, [1.0] * 10 + [3e3] + [1.0] * 15)
+        tops = [max(tops[0], np.abs(rows[:10]).max()), np.abs(rows[10:]).max()]
+        rt.cache8_keep(pool.cache, xpu.Batch(1, 26, 3, dt, up(0, 26), up(6)), up(*([14, 3] + [0] * 24)), up(2))
+        held.update({6: rows[14], 7: rows[3]})
+        assert tops[1] > 8 * tops[0]
+        far(8, [tops[1]])
