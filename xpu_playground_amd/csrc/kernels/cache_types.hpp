@@ -122,13 +122,13 @@ struct RotateArgs {
 };
 
 // An 8-bit cache's positions share scales by blocks of 16: 2^(byte - 127).
-constexpr uint32_t kBlock = 16, kLeastScale = 27, kMostScale = 247;
+constexpr uint32_t kBlock = 16, kLeastScale = 27;
 
 // A sequence's blocks that rows lo .. hi - 1 behind c positions reach.
 XPU_BOTH uint32_t blocks_of(uint32_t n, uint32_t c) { return n ? ((c & (kBlock - 1u)) + n + kBlock - 1u) / kBlock : 0u; }
 
 // The scale byte with which a float of these bits (a finite one, without its
-// sign) is at most 448, the largest code: 1.75 * 2^8.
+// sign) is at most 448, the largest code: 1.75 * 2^8. At most 247.
 XPU_BOTH uint32_t scale_for(uint32_t bits) {
   const uint32_t e = bits >> 23, s = (bits & 0x7fffffu) > 0x600000u ? e + 1u : e;
   return s < kLeastScale + 8u ? kLeastScale : s - 8u;
