@@ -228,7 +228,11 @@ int xpu_cache8_keep(xpu_runtime *rt, const xpu_cache8 *cache, const xpu_batch *b
     if (!batch->n_seqs) return XPU_OK;
     xpu::Keep8Args a{{pool8_of(*cache, 0), batch_of(*batch), kept, counts, new_context}, 1};
     const uint64_t parts = static_cast<uint64_t>(cache->layers) * cache->kv_heads * 2, held = rt->compute_units * 8ull;
-    if (parts * batch->n_seqs > held)  // more blocks than run at once: each takes more, at most 64
+    // more blocks than run at once: each takes more, at most 64 (kernels/cache8.hip).
+    // 48 drafts of 64 nodes, 8 kept: 12.6 us, with a part to a block 41.5; 16: 18 and
+    // 45; 17, from which on a block's parts come one after the other: 37 and 46; 64: 39
+    // and 50
+    if (parts * batch->n_seqs > held)
       a.per_block = static_cast<uint32_t>(4 * std::min<uint64_t>(16, ((parts + 3) / 4 * batch->n_seqs + held - 1) / held));
     const uint64_t groups = (parts + a.per_block - 1) / a.per_block;
     return launch(rt, cache->head_dim == 128 ? "xpu_cache8_keep_d128" : "xpu_cache8_keep_d64", batch->n_seqs * groups, a);

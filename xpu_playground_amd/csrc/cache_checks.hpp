@@ -220,10 +220,12 @@ inline TreePlan tree_plan(const xpu_runtime &rt, bool eight, uint32_t kv_heads, 
   // positions 28.1 and 31.5, behind 16000 19.2 and 23.6). Where more than four
   // fifths of them are row tiles, the chunks get too uneven: three per unit (48
   // single tokens 70.0 us, and 79.8 cut to fit; 32 drafts of up to 8 nodes 53.4
-  // to fit and 56.0). Over 8-bit pages a unit holds three blocks of 32 rows (the
-  // four drafts 297 us, cut for two 345; 48 single tokens 39.5 and 42.5; in 64s,
-  // which leave room for two, 313 and 63), and two per unit do where they do not
-  // fit (48 of 1 .. 26 nodes 46.5 us, with three 51.0).
+  // to fit and 56.0). Over 8-bit pages a unit holds three blocks of 32 rows (whole
+  // calls, cut for three, two and four: the four drafts 290 us, 314 and 313; 48 of
+  // up to 8 nodes 47, 45 and 49; 48 single tokens 45, 42.5 and 49; at D 64 191,
+  // 233 and 172; single tokens 29.9, 27.0 and 29.0, one behind 32000 17.1, 16.1 and
+  // 17.5), and two per unit do where they do not fit (48 of 1 .. 26 nodes: the
+  // kernel 46.5 us, with three 51.0).
   const uint64_t fit = (eight ? 3 : 2) * rt.compute_units / kv_heads;
   if (cut && b.n_seqs <= 64 && row_tiles <= fit * 4 / 5) p.fit = static_cast<uint32_t>(fit);
   p.target = std::max(1u, (eight ? 2 : 3) * rt.compute_units / kv_heads);

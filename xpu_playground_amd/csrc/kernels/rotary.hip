@@ -18,8 +18,8 @@
 //
 // Memory bounds both where there are many rows: 24 prompts of 17 .. 1500 rows,
 // 32 and 8 heads of size 128, 54 us in 16 bits with gains (220 MB, 4.05 TB/s),
-// 53 in 8 bits with half of the dims turned, 65 with all and gains. A step's few
-// rows are one launch and a chain of loads: 48 rows 4.4 us and 8.4, one 7.6.
+// 54 in 8 bits with half of the dims turned, 65 with all and gains. A step's few
+// rows are one launch and a chain of loads: 48 rows 4.4 us and 7.9, one 7.6.
 #include "cache_types.hpp"
 #include "device_common.hpp"
 

@@ -31,11 +31,11 @@
 // which too many tokens would be listed (equal ones, mostly), are the drawing
 // block's alone.
 //
-// 256 rows of 151936 FP32 logits with top-p: 48 us for the first launch, which
+// 256 rows of 151936 FP32 logits with top-p: 50 us for the first launch, which
 // is bound by its 31 vector instructions per token (the reading alone is 31), 33
 // for the second, which reads the row again, 16 for the third, a chain of short
-// steps. One bf16 row with top-k: 4.4, 6.1 and 4.9; 48 rows that ask for all
-// sorts of things 14.5, 12 and 12.
+// steps. One bf16 row with top-k: 4.5, 6.0 and 4.8; 48 rows that ask for all
+// sorts of things 14.3, 12.6 and 13 to 21 (the last by which tokens are asked for).
 #include "device_common.hpp"
 #include "sample_types.hpp"
 

@@ -17,9 +17,10 @@
 // A tile of 32 keys has half the bytes of a 16-bit one. A wavefront takes 32 rows
 // and has two stages of K, one of V (its V goes out once P V has read the last),
 // so three blocks share a CU where blocks of 64 rows with two stages of both
-// leave room for two: four drafts behind 131072 positions 297 us and 313, 48
-// drafts of 1 .. 26 nodes behind 4096 46.5 and 64, 48 single tokens 39.5 and 63,
-// and even 64 drafts of 30 .. 64 nodes 186 and 205. What is left there: without its
+// leave room for two (this kernel alone, without the join): four drafts behind
+// 90000 to 131000 positions 297 us and 313, 48 drafts of 1 .. 26 nodes behind 60 to
+// 8000 46.5 and 64, 48 single tokens 39.5 and 63, and even 64 drafts of 30 .. 64
+// nodes 186 and 205. What is left there: without its
 // arithmetic the four drafts' kernel takes 223 us, without its loads 216, so
 // neither alone bounds it; the copy's rate would be 155.
 #include "attention_core.hpp"
